@@ -153,7 +153,7 @@ def prepare(case, seed):
     s["h"] = torch.empty(T, N, dtype=dt, device=dev)
     if case["op"] == "train":
         s["dh"] = normal(T, N, std=0.1).to(dt)
-        s["g"], s["u"] = torch.empty_like(s["h"]), torch.empty_like(s["h"])
+        s["g"], s["u"] = (torch.empty(T, N, dtype=torch.float32, device=dev) for _ in "gu")
         s["dx"] = torch.empty(T, K, dtype=dt, device=dev)
         s["dwg"], s["dwu"] = torch.empty_like(s["wg"]), torch.empty_like(s["wu"])
         if own:
