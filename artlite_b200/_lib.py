@@ -22,7 +22,9 @@ EXPORTS = ("artlite_moe_last_error", "artlite_moe_version", "artlite_moe_route",
            "artlite_moe_forward",
            "artlite_moe_forward_graph", "artlite_moe_sync", "artlite_moe_debug",
            "artlite_moe_stage_times", "artlite_moe_path", "artlite_moe_weights", "artlite_moe_launch_count", "artlite_moe_destroy",
-           "artlite_moe_ep_unique_id", "artlite_moe_ep_init", "artlite_moe_ep_plan")
+           "artlite_moe_ep_unique_id", "artlite_moe_ep_init", "artlite_moe_ep_plan",
+           "artlite_linear_create", "artlite_linear_forward", "artlite_linear_destroy",
+           "artlite_gated_ffn", "artlite_gated_ffn_work_bytes", "artlite_gated_ffn_backward")
 
 
 class Error(RuntimeError):
@@ -40,6 +42,10 @@ class CapacityError(Error):
 class MoeDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("hidden", "n_experts", "top_k", "expert_ffn", "n_layers", "gating",
                                               "act_dtype", "max_tokens", "device", "path", "ep_rank", "ep_world")]
+
+
+class LinearDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("n_in", "n_out", "qtype", "act_dtype", "activation", "device")]
 
 
 _P, _I64, _I = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
@@ -69,6 +75,12 @@ _SIGS = {
     "artlite_moe_ep_unique_id": ([_P, _I], _I),
     "artlite_moe_ep_init": ([_P, _P, _I], _I),
     "artlite_moe_ep_plan": ([_P, _P, _I, _I, _I, _P, _P, _P, _P], _I),
+    "artlite_linear_create": ([ctypes.POINTER(LinearDesc), _P, _P, ctypes.POINTER(_P)], _I),
+    "artlite_linear_forward": ([_P, _P, _I64, _P, _I64, _I64, _P], _I),
+    "artlite_linear_destroy": ([_P], _I),
+    "artlite_gated_ffn": ([_I, _I, _P, _I64, _P, _P, _P, _I64, _P, _P, _I64, _I, _I, _P], _I),
+    "artlite_gated_ffn_work_bytes": ([_I64, _I], _I64),
+    "artlite_gated_ffn_backward": ([_I, _I, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _I64, _P, _P, _I64, _I, _I, _P], _I),
 }
 
 _lib = None

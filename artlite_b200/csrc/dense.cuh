@@ -1,0 +1,141 @@
+// Shared pieces of the dense products (linear.cu, linear_gemm.cu, ffn.cu, ffn_gemm.cu): activations, argument checks on
+// device buffers, the device status word, and the 4-bit weights' packed layout.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace artlite {
+
+enum { kActNone = -1, kActSilu = 0, kActGelu = 1 };
+
+// ---------------------------------------------------------------- activations
+//
+// silu(z) = z s(z); the tanh-form gelu 0.5 z (1 + tanh(r)), r = sqrt(2 / pi) (z + 0.044715 z^3), is z s(2 r) (since
+// (1 + tanh r) / 2 = s(2 r)), so both are z over 1 + e^-v. EXACT (fp32 outputs): expf and a rounded division; else the
+// fast exponential and division, whose errors (about 2^-21 relative) vanish in a 16-bit result.
+constexpr float kGeluC = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+constexpr float kGeluA = 0.044715f;
+
+template <bool EXACT>
+__device__ __forceinline__ float sigmoid_of(float v) {
+  if constexpr (EXACT) return 1.0f / (1.0f + expf(-v));
+  else return __fdividef(1.0f, 1.0f + __expf(-v));
+}
+template <bool EXACT>
+__device__ __forceinline__ float act_of(int act, float z) {
+  const float v = act == kActGelu ? kGeluC * (z + kGeluA * z * z * z) : z;
+  if constexpr (EXACT) return z / (1.0f + expf(-v));
+  else return __fdividef(z, 1.0f + __expf(-v));
+}
+// act(z) and act'(z) of one z: s (1 + z (1 - s)), or s + z s (1 - s) c (1 + 3 a z^2) with z clamped where the product
+// has long reached 0 (so that 0 times an overflowed square cannot arise)
+__device__ __forceinline__ void act_and_slope(int act, float z, float* a, float* slope) {
+  if (act == kActGelu) {
+    const float zc = fminf(fmaxf(z, -30.0f), 30.0f), z2 = zc * zc;
+    const float s = sigmoid_of<true>(kGeluC * zc * (1.0f + kGeluA * z2));
+    *a = z * s;
+    *slope = s + zc * s * (1.0f - s) * kGeluC * (1.0f + 3.0f * kGeluA * z2);
+  } else {
+    const float s = sigmoid_of<true>(z);
+    *a = z * s;
+    *slope = s * (1.0f + z * (1.0f - s));
+  }
+}
+
+// 2^n, -126 <= n <= 127
+__device__ __forceinline__ float pow2(int n) { return __int_as_float((n + 127) << 23); }
+
+// ---------------------------------------------------------------- 16-bit types
+
+template <class T>
+struct Num;
+template <>
+struct Num<__nv_bfloat16> {
+  static __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+  }
+};
+template <>
+struct Num<__half> {
+  static __device__ __forceinline__ float up(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half down(float v) { return __float2half_rn(v); }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  }
+};
+template <>
+struct Num<float> {
+  static __device__ __forceinline__ float up(float v) { return v; }
+  static __device__ __forceinline__ float down(float v) { return v; }
+};
+
+// ---------------------------------------------------------------- the 4-bit weights' packed layout
+//
+// A matrix of N rows of K values is held as tiles of 16 rows x 256 values (K padded to 256 with zero scales, the rows
+// to 128), tile after tile along a row group, every tile one block of bytes:
+//   codes   [unit u of 64 values][lane = 4 g + t][16 B]: of row g and row g + 8, the values 64 u + 32 j + 8 t .. + 7 of
+//           the unit's two 32-value groups j. Word s = 2 j + h of the 16 bytes holds both rows' values 32 j + 8 t + 4 h
+//           .. + 3 as the eight nibbles of one mma.sync m16n8k16 step's A fragment (a0 = row g's first pair, a1 = row
+//           g + 8's, a2, a3 the second pairs): pair i in nibbles i and i + 4, so that (w >> 4 i) & 0x000F000F is the
+//           pair (IQ4_NL: in byte i, a 256-entry table's index). The k order inside a group is free as long as x follows
+//           it: lane t's x is eight consecutive values, and a step's sum stays inside one group.
+//   scales  [lane = 4 g + t] unit t's: Q4_0 / IQ4_NL 8 B: fp16 d of row g's two 32-value groups, then of row g + 8's;
+//           Q4_1 16 B: those and the same of m; Q4_K 8 B: for row g, then for row g + 8, a word of sc | mn << 6 of both
+//           groups in 24 bits and byte t of (d | dmin << 16) above.
+// The bytes of a tile are the raw blocks' (2304 for 4096 values of Q4_0, Q4_K, IQ4_NL; 2560 for Q4_1).
+constexpr int kTileRows = 16, kTileK = 256, kUnits = 4, kCodeBytes = 2048;
+constexpr int kPadTiles = 8;  // row tiles are padded to whole 128-row groups
+__host__ __device__ constexpr int scale_bytes(int qt) { return qt == ARTLITE_Q4_1 ? 512 : 256; }
+__host__ __device__ constexpr int tile_bytes(int qt) { return kCodeBytes + scale_bytes(qt); }
+
+// ---------------------------------------------------------------- host side
+
+// makes `dev` current for a scope
+struct DeviceScope {
+  int prev = -1;
+  int code = ARTLITE_OK;
+  explicit DeviceScope(int dev) {
+    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+    if (prev != dev && cudaSetDevice(dev) != cudaSuccess) {
+      cudaGetLastError();
+      set_error("device %d is not available", dev);
+      code = ARTLITE_ECUDA;
+      prev = -1;
+    } else if (prev == dev) {
+      prev = -1;
+    }
+  }
+  ~DeviceScope() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+};
+
+// the device that owns p (device or managed memory), -1 for host memory
+int device_of(const void* p);
+
+// The status word the dense kernels of device `dev` report a run-out wait in: mapped host memory, so that the host
+// reads it without a copy or a wait. take_dense_status returns and clears what an earlier call left.
+int dense_status(int dev, DevStatus** out);
+int take_dense_status(int dev, const char* who);
+
+// SMs of device `dev`
+int sm_count(int dev, int* out);
+
+}  // namespace artlite

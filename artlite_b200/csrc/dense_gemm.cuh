@@ -1,0 +1,88 @@
+// What the dense tensor-core products (linear_gemm.cu, ffn_gemm.cu) share: the tile of a CTA pair, the order of the
+// tiles, the tensor maps, the epilogue's stores and the kernel's beginning and end.
+//
+// A pair of CTAs on two SMs (cta_group::2) computes a tile of 256 x 256: 256 rows of A (128 a CTA) by 256 columns (each
+// CTA brings half of B), K in stages of 64, fp32 accumulators in TMEM, two of 256 columns, so that one tile's epilogue
+// runs under the next one's MMAs. A pair's tile reads (256 + 256) x 64 values a stage for 256 x 256 x 64 products: half
+// the operand traffic a product of one-CTA tiles of 128 x 256.
+#pragma once
+
+#include "dense.cuh"
+#include "umma.cuh"
+
+namespace artlite {
+namespace dg {
+
+constexpr int BK = 64, HALF = 128, TILE = 256;
+constexpr int kStageBytes = HALF * BK * 2;  // one operand's half tile
+
+// tiles in groups of 8 rows of tiles: the pairs that run at one time share few rows and columns of operands in L2
+struct TileOrder {
+  int tm, tn;
+};
+__device__ __forceinline__ void tile_at(const TileOrder& o, int id, int* m, int* n) {
+  constexpr int G = 8;
+  const int per = G * o.tn, grp = id / per, rem = id - grp * per;
+  const int gm = min(G, o.tm - grp * G);
+  *n = rem / gm;
+  *m = grp * G + (rem - *n * gm);
+}
+
+// 32 consecutive values of an output row: 16-byte stores where the row allows them (vec) and all are inside
+template <class T>
+__device__ __forceinline__ void store32(T* dst, const float (&v)[32], int valid, bool vec) {
+  if (valid <= 0) return;
+  if (vec && valid >= 32) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int c = 0; c < 8; c++)
+        reinterpret_cast<float4*>(dst)[c] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+        reinterpret_cast<uint4*>(dst)[c] =
+            make_uint4(Num<T>::pack(v[8 * c], v[8 * c + 1]), Num<T>::pack(v[8 * c + 2], v[8 * c + 3]),
+                       Num<T>::pack(v[8 * c + 4], v[8 * c + 5]), Num<T>::pack(v[8 * c + 6], v[8 * c + 7]));
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 32; j++)
+    if (j < valid) dst[j] = Num<T>::down(v[j]);
+}
+
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* slot) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(slot)), "r"(512));
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free_pair(uint32_t tmem) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+}
+
+// a 2D map of rows x cols 16-bit values, ld apart, boxes of box_x x box_y, 128-byte swizzle, zeros outside
+// (dense_gemm's host side: linear_gemm.cu)
+int make_operand_map(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int64_t ld, int box_x, int box_y);
+
+// a launch of `pairs` CTA pairs
+template <class K, class P>
+int launch_pairs(K kern, const P& p, int pairs, int threads, size_t smem, cudaStream_t st) {
+  AL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(2 * pairs));
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  AL_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
+  count_launch();
+  return ARTLITE_OK;
+}
+
+}  // namespace dg
+}  // namespace artlite

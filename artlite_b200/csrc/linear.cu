@@ -1,0 +1,460 @@
+// The product with a 4-bit GGUF matrix outside an expert (artlite_linear_*): the handle, the packing of the raw blocks
+// into the fragment layout of dense.cuh, and the choice of kernel. A forward keeps nothing in the handle: any number of
+// them may run at once, on any streams, captured or not.
+#include <cuda_runtime.h>
+#include <math.h>
+
+#include <memory>
+#include <mutex>
+#include <new>
+
+#include "kernels.cuh"
+#include "linear.cuh"
+#include "quant.cuh"
+#include "small_batch.cuh"
+
+namespace artlite {
+
+// ---------------------------------------------------------------- host helpers of the dense products
+
+namespace {
+
+constexpr int kMaxDevices = 64;
+std::mutex g_mu;
+DevStatus* g_status[kMaxDevices] = {};
+cudaMemPool_t g_pool[kMaxDevices] = {};
+int g_sms[kMaxDevices] = {};
+
+// lets this thread allocate while another of the process's streams is being captured
+struct RelaxedCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
+}  // namespace
+
+int device_of(const void* p) {
+  cudaPointerAttributes at;
+  if (!p || cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+    cudaGetLastError();
+    return -1;
+  }
+  return at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged ? at.device : -1;
+}
+
+int dense_status(int dev, DevStatus** out) {
+  AL_CHECK(dev >= 0 && dev < kMaxDevices, ARTLITE_EUNSUPPORTED, "device %d (at most %d)", dev, kMaxDevices);
+  std::lock_guard<std::mutex> lock(g_mu);
+  if (!g_status[dev]) {
+    RelaxedCapture relaxed;
+    void* p = nullptr;
+    AL_CUDA(cudaHostAlloc(&p, sizeof(DevStatus), cudaHostAllocMapped | cudaHostAllocPortable));
+    *static_cast<DevStatus*>(p) = DevStatus{};
+    g_status[dev] = static_cast<DevStatus*>(p);
+  }
+  *out = g_status[dev];
+  return ARTLITE_OK;
+}
+
+int take_dense_status(int dev, const char* who) {
+  DevStatus* s;
+  AL_TRY(dense_status(dev, &s));
+  volatile DevStatus* v = s;
+  const int code = v->code;
+  if (code == 0) return ARTLITE_OK;
+  const int site = v->a, block = v->b;
+  v->code = 0;
+  set_error("%s: an earlier call's bounded device wait ran out (site %d, block %d)", who, site, block);
+  return code;
+}
+
+int sm_count(int dev, int* out) {
+  AL_CHECK(dev >= 0 && dev < kMaxDevices, ARTLITE_EUNSUPPORTED, "device %d (at most %d)", dev, kMaxDevices);
+  std::lock_guard<std::mutex> lock(g_mu);
+  if (!g_sms[dev]) AL_CUDA(cudaDeviceGetAttribute(&g_sms[dev], cudaDevAttrMultiProcessorCount, dev));
+  *out = g_sms[dev];
+  return ARTLITE_OK;
+}
+
+int stream_alloc(int dev, size_t n, cudaStream_t st, void** out) {
+  AL_CHECK(dev >= 0 && dev < kMaxDevices, ARTLITE_EUNSUPPORTED, "device %d (at most %d)", dev, kMaxDevices);
+  cudaMemPool_t pool;
+  {
+    std::lock_guard<std::mutex> lock(g_mu);
+    if (!g_pool[dev]) {
+      RelaxedCapture relaxed;
+      cudaMemPoolProps props{};
+      props.allocType = cudaMemAllocationTypePinned;
+      props.location.type = cudaMemLocationTypeDevice;
+      props.location.id = dev;
+      cudaMemPool_t p;
+      AL_CUDA(cudaMemPoolCreate(&p, &props));
+      uint64_t keep = ~0ull;  // (freed blocks stay in the pool: the next call pays no mapping)
+      AL_CUDA(cudaMemPoolSetAttribute(p, cudaMemPoolAttrReleaseThreshold, &keep));
+      g_pool[dev] = p;
+    }
+    pool = g_pool[dev];
+  }
+  AL_CUDA(cudaMallocFromPoolAsync(out, n, pool, st));
+  return ARTLITE_OK;
+}
+
+int stream_free(void* p, cudaStream_t st) {
+  AL_CUDA(cudaFreeAsync(p, st));
+  return ARTLITE_OK;
+}
+
+// ---------------------------------------------------------------- packing
+
+namespace {
+
+__device__ __forceinline__ int code_at(int qt, const uint8_t* row, int k) {
+  if (qt == ARTLITE_Q4_K) {
+    const uint8_t* b = row + (int64_t)(k >> 8) * 144 + 16;
+    const int g = (k >> 5) & 7, c = b[32 * (g >> 1) + (k & 31)];
+    return g & 1 ? c >> 4 : c & 15;
+  }
+  const uint8_t* b = row + (int64_t)(k >> 5) * (qt == ARTLITE_Q4_1 ? 20 : 18) + (qt == ARTLITE_Q4_1 ? 4 : 2);
+  const int i = k & 31, c = b[i & 15];
+  return i < 16 ? c & 15 : c >> 4;
+}
+
+__device__ __forceinline__ uint32_t half_bits(float v) { return __half_as_ushort(__float2half_rn(v)); }
+
+// the largest magnitude any scale, minimum or value of the matrix has, as fp32 bits (non-negative floats order as ints)
+__global__ void weight_bound_kernel(int qt, const uint8_t* raw, int64_t rb, int64_t N, int K, uint32_t* bound) {
+  const int groups = K / 32;
+  float m = 0.0f;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < N * groups; i += (int64_t)gridDim.x * blockDim.x) {
+    const uint8_t* row = raw + (i / groups) * rb;
+    const int g = (int)(i % groups);
+    if (qt == ARTLITE_Q4_K) {
+      const uint8_t* b = row + (int64_t)(g >> 3) * 144;
+      int sc, mn;
+      k_scale_min(b, g & 7, &sc, &mn);
+      const float d = fabsf(f16_at(b)), dm = fabsf(f16_at(b + 2));
+      m = fmaxf(m, fmaxf(fmaxf(d, dm), fmaxf(15.0f * d * sc, dm * mn) + fminf(15.0f * d * sc, dm * mn)));
+    } else if (qt == ARTLITE_Q4_1) {
+      const uint8_t* b = row + (int64_t)g * 20;
+      m = fmaxf(m, 15.0f * fabsf(f16_at(b)) + fabsf(f16_at(b + 2)));
+    } else {
+      m = fmaxf(m, (qt == ARTLITE_IQ4_NL ? 127.0f : 8.0f) * fabsf(f16_at(row + (int64_t)g * 18)));
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  if ((threadIdx.x & 31) == 0) atomicMax(bound, __float_as_uint(m));
+}
+
+// one warp a packed tile (dense.cuh); scale: 2^w_exp
+__global__ void pack_kernel(int qt, const uint8_t* raw, int64_t rb, int64_t N, int K, int64_t row_tiles, int chunks,
+                            float scale, uint8_t* out) {
+  const int64_t tile = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (tile >= row_tiles * chunks) return;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int64_t mt = tile / chunks;
+  const int ch = (int)(tile % chunks);
+  uint8_t* o = out + tile * tile_bytes(qt);
+  const uint8_t* row[2];
+  for (int r = 0; r < 2; r++) {
+    const int64_t n = mt * kTileRows + g + 8 * r;
+    row[r] = n < N ? raw + n * rb : nullptr;
+  }
+  for (int u = 0; u < kUnits; u++) {
+    uint32_t w[4];
+    for (int s = 0; s < 4; s++) {
+      const int k = kTileK * ch + 64 * u + 32 * (s >> 1) + 8 * t + 4 * (s & 1);
+      uint32_t v = 0;
+      for (int i = 0; i < 4; i++) {  // pair i: row i & 1, values 2 (i >> 1) and + 1
+        for (int e = 0; e < 2; e++) {
+          const int kk = k + 2 * (i >> 1) + e;
+          const uint32_t c = row[i & 1] && kk < K ? (uint32_t)code_at(qt, row[i & 1], kk) : 0u;
+          v |= c << (qt == ARTLITE_IQ4_NL ? 8 * i + 4 * e : 4 * i + 16 * e);
+        }
+      }
+      w[s] = v;
+    }
+    reinterpret_cast<uint4*>(o)[32 * u + lane] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  // lane 4 g + t: unit t's scales
+  uint32_t s[4] = {0, 0, 0, 0};
+  for (int r = 0; r < 2; r++) {
+    if (!row[r]) continue;
+    if (qt == ARTLITE_Q4_K) {
+      if (kTileK * ch >= K) continue;
+      const uint8_t* b = row[r] + (int64_t)ch * 144;
+      uint32_t v = 0;
+      for (int j = 0; j < 2; j++) {
+        int sc, mn;
+        k_scale_min(b, 2 * t + j, &sc, &mn);
+        v |= (uint32_t)(sc | mn << 6) << (12 * j);
+      }
+      const uint32_t dd = half_bits(f16_at(b) * scale) | half_bits(f16_at(b + 2) * scale) << 16;
+      s[r] = v | ((dd >> (8 * t)) & 0xFFu) << 24;
+    } else {
+      const int size = qt == ARTLITE_Q4_1 ? 20 : 18;
+      for (int j = 0; j < 2; j++) {
+        const int k = kTileK * ch + 64 * t + 32 * j;
+        if (k >= K) continue;
+        const uint8_t* b = row[r] + (int64_t)(k >> 5) * size;
+        s[r] |= half_bits(f16_at(b) * scale) << (16 * j);
+        if (qt == ARTLITE_Q4_1) s[2 + r] |= half_bits(f16_at(b + 2) * scale) << (16 * j);
+      }
+    }
+  }
+  if (qt == ARTLITE_Q4_1) reinterpret_cast<uint4*>(o + kCodeBytes)[lane] = make_uint4(s[0], s[1], s[2], s[3]);
+  else reinterpret_cast<uint2*>(o + kCodeBytes)[lane] = make_uint2(s[0], s[1]);
+}
+
+// x's rows as scaled fp16 (linear.cuh): a CTA a row
+__global__ void half_rows_kernel(const uint16_t* x, int64_t ldx, int K, uint16_t* out, int32_t* row_exp) {
+  const uint16_t* row = x + (int64_t)blockIdx.x * ldx;
+  __shared__ float part[8];
+  float m = 0.0f;
+  for (int k = 8 * threadIdx.x; k < K; k += 8 * blockDim.x) {
+    const uint4 v = *reinterpret_cast<const uint4*>(row + k);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float2 f = Num<__nv_bfloat16>::unpack(w[i]);
+      m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
+  __syncthreads();
+  m = part[0];
+  for (int i = 1; i < (int)(blockDim.x >> 5); i++) m = fmaxf(m, part[i]);
+  // (a row of zeros, or with an infinity, stays as it is: fp16 has both)
+  const int e = m > 0.0f && m < __int_as_float(0x7F800000) ? ilogbf(m) - 14 : 0;
+  const float s0 = pow2(-e / 2), s1 = pow2(-e + e / 2);  // (2^-e may exceed fp32's range)
+  if (threadIdx.x == 0) row_exp[blockIdx.x] = e;
+  for (int k = 8 * threadIdx.x; k < K; k += 8 * blockDim.x) {
+    const uint4 v = *reinterpret_cast<const uint4*>(row + k);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float2 f = Num<__nv_bfloat16>::unpack(w[i]);
+      o[i] = Num<__half>::pack(f.x * s0 * s1, f.y * s0 * s1);
+    }
+    *reinterpret_cast<uint4*>(out + (int64_t)blockIdx.x * K + k) = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+bool linear_type(int qt) {
+  return qt == ARTLITE_Q4_0 || qt == ARTLITE_Q4_1 || qt == ARTLITE_Q4_K || qt == ARTLITE_IQ4_NL;
+}
+
+}  // namespace
+
+int launch_half_rows(const uint16_t* x, int64_t ldx, int64_t T, int K, uint16_t* out, int32_t* row_exp, cudaStream_t st) {
+  half_rows_kernel<<<(unsigned)T, 256, 0, st>>>(x, ldx, K, out, row_exp);
+  AL_LAUNCHED();
+  return ARTLITE_OK;
+}
+
+}  // namespace artlite
+
+using namespace artlite;
+
+struct artlite_linear {
+  artlite_linear_desc d;
+  int dev = 0;
+  bool gated = false;
+  int w_exp[2] = {0, 0};
+  DevBuf w[2];
+  DevStatus* status = nullptr;
+};
+
+namespace {
+
+size_t elem(int dtype) { return dtype == ARTLITE_F32 ? 4 : 2; }
+
+// the raw rows (host or device) into w's packed tiles; waits for the copy
+int pack(artlite_linear* h, int which, const void* raw) {
+  const int qt = h->d.qtype, K = h->d.n_in;
+  const int64_t N = h->d.n_out;
+  const int64_t rb = (int64_t)K / q_per(qt) * q_bytes(qt);
+  DevBuf stage, bound;
+  const uint8_t* src = static_cast<const uint8_t*>(raw);
+  if (device_of(raw) != h->dev) {
+    AL_TRY(stage.reserve((size_t)(N * rb)));
+    AL_CUDA(cudaMemcpy(stage.ptr, raw, (size_t)(N * rb), cudaMemcpyDefault));
+    src = stage.as<uint8_t>();
+  }
+  AL_TRY(bound.reserve(4));
+  AL_CUDA(cudaMemset(bound.ptr, 0, 4));
+  weight_bound_kernel<<<1024, 256>>>(qt, src, rb, N, K, bound.as<uint32_t>());
+  AL_LAUNCHED();
+  float m;
+  AL_CUDA(cudaMemcpy(&m, bound.ptr, 4, cudaMemcpyDeviceToHost));
+  // the packed scales are the file's times 2^w_exp: the largest value below 2^15, so that the prompt kernel's fp16
+  // weights cannot overflow and only values 2^-29 below the largest lose bits
+  int e = 0;
+  if (m > 0.0f && isfinite(m)) e = 14 - ilogbf(m);
+  h->w_exp[which] = e;
+  const int chunks = (int)cdiv(K, kTileK);
+  const int64_t row_tiles = cdiv(N, kTileRows * kPadTiles) * kPadTiles;
+  AL_TRY(h->w[which].reserve((size_t)(row_tiles * chunks * tile_bytes(qt))));
+  pack_kernel<<<(unsigned)cdiv(row_tiles * chunks, 8), 256>>>(qt, src, rb, N, K, row_tiles, chunks, ldexpf(1.0f, e),
+                                                                h->w[which].as<uint8_t>());
+  AL_LAUNCHED();
+  AL_CUDA(cudaDeviceSynchronize());
+  return ARTLITE_OK;
+}
+
+template <int QT, class XT, bool VEC>
+int small(const sb::Args& a, bool gated, cudaStream_t st) {
+  return gated ? sb::launch<sb::Quant<QT>, XT, true, VEC>(a, st) : sb::launch<sb::Quant<QT>, XT, false, VEC>(a, st);
+}
+template <class XT, bool VEC>
+int small_of(int qt, const sb::Args& a, bool gated, cudaStream_t st) {
+  switch (qt) {
+    case ARTLITE_Q4_0: return small<ARTLITE_Q4_0, XT, VEC>(a, gated, st);
+    case ARTLITE_Q4_1: return small<ARTLITE_Q4_1, XT, VEC>(a, gated, st);
+    case ARTLITE_Q4_K: return small<ARTLITE_Q4_K, XT, VEC>(a, gated, st);
+    default: return small<ARTLITE_IQ4_NL, XT, VEC>(a, gated, st);
+  }
+}
+
+// tokens up to which the small-batch kernel runs
+constexpr int64_t kSmallTokens = 32;
+
+int run(const artlite_linear* h, const void* x, int64_t ldx, void* y, int64_t ldy, int64_t T, cudaStream_t st) {
+  const artlite_linear_desc& d = h->d;
+  // 16-byte loads of x need its rows 16-byte aligned
+  const bool vec = ((uintptr_t)x % 16) == 0 && (ldx * (int64_t)elem(d.act_dtype)) % 16 == 0;
+  if (T > kSmallTokens && d.act_dtype != ARTLITE_F32 && vec) {
+    LinearGemmArgs g{};
+    g.qtype = d.qtype;
+    g.w0 = h->w[0].as<uint8_t>();
+    g.w1 = h->w[1].as<uint8_t>();
+    g.w_exp0 = h->w_exp[0];
+    g.w_exp1 = h->w_exp[1];
+    g.x = static_cast<const uint16_t*>(x);
+    g.ldx = ldx;
+    g.y = y;
+    g.ldy = ldy;
+    g.out_dtype = d.act_dtype;
+    g.T = T;
+    g.K = d.n_in;
+    g.N = d.n_out;
+    g.gated = h->gated;
+    g.act = d.activation;
+    g.status = h->status;
+    if (d.act_dtype == ARTLITE_F16) return launch_linear_gemm(g, st);
+    const size_t xb = ((size_t)T * d.n_in * 2 + 255) & ~(size_t)255;
+    void* ws = nullptr;
+    AL_TRY(stream_alloc(h->dev, xb + (size_t)T * 4, st, &ws));
+    int32_t* ex = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(ws) + xb);
+    int rc = launch_half_rows(g.x, ldx, T, d.n_in, static_cast<uint16_t*>(ws), ex, st);
+    g.x = static_cast<const uint16_t*>(ws);
+    g.ldx = d.n_in;
+    g.row_exp = ex;
+    if (rc == ARTLITE_OK) rc = launch_linear_gemm(g, st);
+    const int rf = stream_free(ws, st);
+    return rc != ARTLITE_OK ? rc : rf;
+  }
+  sb::Args a{};
+  a.w0 = h->w[0].ptr;
+  a.w1 = h->w[1].ptr;
+  a.x = x;
+  a.y = y;
+  a.ldx = ldx;
+  a.ldy = ldy;
+  a.T = T;
+  a.K = d.n_in;
+  a.N = d.n_out;
+  a.act = d.activation;
+  a.scale0 = ldexpf(1.0f, -h->w_exp[0]);
+  a.scale1 = ldexpf(1.0f, -h->w_exp[1]);
+  if (d.act_dtype == ARTLITE_F32)
+    return vec ? small_of<float, true>(d.qtype, a, h->gated, st) : small_of<float, false>(d.qtype, a, h->gated, st);
+  if (d.act_dtype == ARTLITE_F16)
+    return vec ? small_of<__half, true>(d.qtype, a, h->gated, st) : small_of<__half, false>(d.qtype, a, h->gated, st);
+  return vec ? small_of<__nv_bfloat16, true>(d.qtype, a, h->gated, st)
+             : small_of<__nv_bfloat16, false>(d.qtype, a, h->gated, st);
+}
+
+}  // namespace
+
+extern "C" {
+#pragma GCC visibility push(default)
+
+int artlite_linear_create(const artlite_linear_desc* desc, const void* w, const void* w_up, artlite_linear** out) {
+  AL_CHECK(desc && out, ARTLITE_EINVAL, "linear: null argument");
+  *out = nullptr;
+  const artlite_linear_desc& d = *desc;
+  AL_CHECK(linear_type(d.qtype), ARTLITE_EUNSUPPORTED, "linear: GGUF type %s (Q4_0, Q4_1, Q4_K and IQ4_NL are read)",
+           qtype_name(d.qtype));
+  AL_CHECK(d.n_in >= 1 && d.n_out >= 1 && d.n_in <= (1 << 24) && d.n_in % q_per(d.qtype) == 0, ARTLITE_EINVAL,
+           "linear: %d values a row, %d rows (rows are whole blocks of %d values)", d.n_in, d.n_out, q_per(d.qtype));
+  AL_CHECK(d.act_dtype == ARTLITE_F32 || d.act_dtype == ARTLITE_F16 || d.act_dtype == ARTLITE_BF16, ARTLITE_EINVAL,
+           "linear: activation type %d", d.act_dtype);
+  AL_CHECK(!w_up || d.activation == kActSilu || d.activation == kActGelu, ARTLITE_EINVAL, "linear: activation %d",
+           d.activation);
+  AL_CHECK(w, ARTLITE_EINVAL, "linear: null weights");
+  int dev = d.device, cur;
+  AL_CUDA(cudaGetDevice(&cur));
+  if (dev < 0) dev = cur;
+  DeviceScope scope(dev);
+  AL_TRY(scope.code);
+  std::unique_ptr<artlite_linear> h(new (std::nothrow) artlite_linear);
+  AL_CHECK(h, ARTLITE_ECUDA, "linear: out of host memory");
+  h->d = d;
+  h->dev = dev;
+  h->gated = w_up != nullptr;
+  AL_TRY(dense_status(dev, &h->status));
+  int rc = pack(h.get(), 0, w);
+  if (rc == ARTLITE_OK && w_up) rc = pack(h.get(), 1, w_up);
+  if (rc != ARTLITE_OK) {
+    cudaGetLastError();  // (a failed allocation is reported here, not by the next launch)
+    return rc;
+  }
+  *out = h.release();
+  return ARTLITE_OK;
+}
+
+int artlite_linear_forward(const artlite_linear* h, const void* x, int64_t ldx, void* y, int64_t ldy, int64_t T,
+                           void* stream) {
+  AL_CHECK(h, ARTLITE_EINVAL, "linear: null handle");
+  const artlite_linear_desc& d = h->d;
+  AL_CHECK(T >= 0 && T <= 0x7FFFFFFF && ldx >= d.n_in && ldy >= d.n_out, ARTLITE_EINVAL,
+           "linear: T %lld, rows of x %lld and of y %lld apart (%d and %d values)", (long long)T, (long long)ldx,
+           (long long)ldy, d.n_in, d.n_out);
+  if (T == 0) return ARTLITE_OK;
+  AL_CHECK(x && y, ARTLITE_EINVAL, "linear: null array");
+  const size_t e = elem(d.act_dtype);
+  AL_CHECK((uintptr_t)x % e == 0 && (uintptr_t)y % e == 0, ARTLITE_EINVAL, "linear: x or y is not aligned to its values");
+  const int dx = device_of(x), dy = device_of(y);
+  AL_CHECK((dx < 0) == (dy < 0), ARTLITE_EINVAL, "linear: one of x and y is host memory, the other device memory");
+  AL_CHECK(dx < 0 || (dx == h->dev && dy == h->dev), ARTLITE_EINVAL, "linear: x on device %d, y on device %d, weights on %d",
+           dx, dy, h->dev);
+  DeviceScope scope(h->dev);
+  AL_TRY(scope.code);
+  AL_TRY(take_dense_status(h->dev, "linear"));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dx >= 0) return run(h, x, ldx, y, ldy, T, st);
+  // host arrays: staged, and the call returns when y is back
+  DevBuf bx, by;
+  AL_TRY(bx.reserve((size_t)T * d.n_in * e));
+  AL_TRY(by.reserve((size_t)T * d.n_out * e));
+  AL_CUDA(cudaMemcpy2DAsync(bx.ptr, d.n_in * e, x, ldx * e, d.n_in * e, (size_t)T, cudaMemcpyDefault, st));
+  AL_TRY(run(h, bx.ptr, d.n_in, by.ptr, d.n_out, T, st));
+  AL_CUDA(cudaMemcpy2DAsync(y, ldy * e, by.ptr, d.n_out * e, d.n_out * e, (size_t)T, cudaMemcpyDefault, st));
+  AL_CUDA(cudaStreamSynchronize(st));
+  return take_dense_status(h->dev, "linear");
+}
+
+int artlite_linear_destroy(artlite_linear* h) {
+  if (!h) return ARTLITE_OK;
+  DeviceScope scope(h->dev);
+  delete h;
+  return ARTLITE_OK;
+}
+
+#pragma GCC visibility pop
+}  // extern "C"

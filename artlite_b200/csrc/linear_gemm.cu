@@ -1,0 +1,410 @@
+// The product with a 4-bit matrix for prompts, on the 5th-generation tensor cores: y = x . W^T, or the gated pair
+// act(x Wg^T) (x Wu^T) with both products, the activation and the product in one kernel.
+//
+// Tile (dense_gemm.cuh): 256 token rows (A, fp16, TMA) x 256 weight rows (B), a CTA pair. Linear: 256 output features;
+// gated: the 128 gate rows (CTA 0's half of B) and the 128 up rows (CTA 1's half) of 128 features, so that a token's
+// gate and up values lie in one TMEM lane and the epilogue needs no exchange. B is decoded from the packed tiles
+// (dense.cuh) straight into the UMMA layout: a bulk copy brings eight tiles (128 rows x 256 values), eight warps turn a
+// tile each and 64 values at a time into fp16.
+//
+// The operands are fp16 for either activation type: a code times its group's scale rounds once to 11 significant bits
+// (bf16 would keep 8: a bf16 weight's rounding alone is as large as the output's, measured 0.0024 against 0.0017 of the
+// result's norm). bf16 x fits after a row's values are multiplied by a power of two (linear.cu half_rows_kernel); fp16's
+// range then loses only what is 2^-29 below a row's largest value. The packed scales carry a power of two too; the
+// epilogue undoes both.
+//
+// Warps: 0 the token rows' TMA, 1 the MMAs (the leader CTA's), 2 the packed tiles' copies, 3 idle, 4 - 7 the epilogue,
+// 8 - 15 the decoding.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "dense_gemm.cuh"
+#include "linear.cuh"
+
+namespace artlite {
+namespace {
+
+using namespace dg;
+
+constexpr int S = 5, R = 2;
+constexpr int kThreads = 512;
+constexpr int kDecodeWarps = 8;
+
+struct Params {
+  CUtensorMap map_x;
+  const uint8_t* w[2];
+  int64_t row_tiles;  // padded row tiles of a matrix
+  void* y;
+  int64_t ldy;
+  const int32_t* row_exp;
+  int w_exp0, w_exp1;
+  int T, K, N;
+  int act;
+  bool vec_y;
+  TileOrder order;
+  DevStatus* status;
+};
+
+struct Smem {
+  uint64_t full_a[S], full_b[S], empty[S], raw_full[R], raw_empty[R], tfull[2], tempty[2];
+  uint32_t tmem_base;
+  int abort;
+};
+
+template <int QT>
+constexpr size_t smem_bytes() {
+  return 1024 + 2 * (size_t)S * kStageBytes + (size_t)R * 8 * tile_bytes(QT) + sizeof(Smem) +
+         (QT == ARTLITE_IQ4_NL ? 256 * 4 : 0) + 64;
+}
+
+__device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   tc::smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
+               : "memory");
+}
+
+__device__ __forceinline__ __half2 h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+__device__ __forceinline__ uint32_t u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+
+// a unit's scales (and minima) of row r, group j, doubled into pairs
+template <int QT>
+struct Scales {
+  __half2 d[2][2], m[2][2];
+  __device__ __forceinline__ void load(const uint8_t* tile, int g, int u) {
+    const uint8_t* p = tile + kCodeBytes;
+    if constexpr (QT == ARTLITE_Q4_1) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[4 * g + u];
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        d[r][0] = __low2half2(h2(w[r])), d[r][1] = __high2half2(h2(w[r]));
+        m[r][0] = __low2half2(h2(w[2 + r])), m[r][1] = __high2half2(h2(w[2 + r]));
+      }
+    } else if constexpr (QT == ARTLITE_Q4_K) {
+      uint2 v[4];
+#pragma unroll
+      for (int t = 0; t < 4; t++) v[t] = reinterpret_cast<const uint2*>(p)[4 * g + t];
+      const uint2 mine = u == 0 ? v[0] : u == 1 ? v[1] : u == 2 ? v[2] : v[3];
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        const uint32_t dd = r ? (v[0].y >> 24) | (v[1].y >> 24) << 8 | (v[2].y >> 24) << 16 | (v[3].y & 0xFF000000u)
+                              : (v[0].x >> 24) | (v[1].x >> 24) << 8 | (v[2].x >> 24) << 16 | (v[3].x & 0xFF000000u);
+        const float2 f = __half22float2(h2(dd));
+        const uint32_t w = r ? mine.y : mine.x;
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          // (the products of the file's fp16 and 6-bit scales round to fp16: 2^-12 of a weight, against the output's
+          // 2^-9 in bf16)
+          d[r][j] = __float2half2_rn(f.x * (float)((w >> (12 * j)) & 63u));
+          m[r][j] = __float2half2_rn(-f.y * (float)((w >> (12 * j + 6)) & 63u));
+        }
+      }
+    } else {
+      const uint2 v = reinterpret_cast<const uint2*>(p)[4 * g + u];
+      d[0][0] = __low2half2(h2(v.x)), d[0][1] = __high2half2(h2(v.x));
+      d[1][0] = __low2half2(h2(v.y)), d[1][1] = __high2half2(h2(v.y));
+    }
+  }
+};
+
+// word w's pair i (row i & 1) with its group's scale: one rounding to fp16 from the exact code
+template <int QT>
+__device__ __forceinline__ uint32_t decode_pair(uint32_t w, int i, __half2 d, __half2 m, const uint32_t* table) {
+  if constexpr (QT == ARTLITE_IQ4_NL) {
+    return u32(__hmul2(h2(table[(w >> (8 * i)) & 0xFFu]), d));
+  } else {
+    const __half2 q = __hsub2(h2(((w >> (4 * i)) & 0x000F000Fu) | 0x64006400u),
+                              h2(QT == ARTLITE_Q4_0 ? 0x64086408u : 0x64006400u));
+    if constexpr (QT == ARTLITE_Q4_0) return u32(__hmul2(q, d));
+    else return u32(__hfma2(q, d, m));
+  }
+}
+
+template <int QT, class T, bool GATED>
+__global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant__ Params p) {
+  constexpr int TB = tile_bytes(QT);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* sA = base;
+  uint8_t* sB = sA + S * kStageBytes;
+  uint8_t* sR = sB + S * kStageBytes;
+  Smem* sm = reinterpret_cast<Smem*>(sR + R * 8 * TB);
+  uint32_t* table = reinterpret_cast<uint32_t*>(sm + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t crank = tc::cluster_rank();
+  const int total = p.order.tm * p.order.tn, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int ksteps = (p.K + BK - 1) / BK, chunks = (p.K + kTileK - 1) / kTileK;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; i++) {
+      tc::mbar_init(&sm->full_a[i], 1);
+      tc::mbar_init(&sm->full_b[i], 2 * kDecodeWarps);
+      tc::mbar_init(&sm->empty[i], 1);
+    }
+    for (int i = 0; i < R; i++) {
+      tc::mbar_init(&sm->raw_full[i], 1);
+      tc::mbar_init(&sm->raw_empty[i], kDecodeWarps);
+    }
+    for (int i = 0; i < 2; i++) {
+      tc::mbar_init(&sm->tfull[i], 1);
+      tc::mbar_init(&sm->tempty[i], 2 * 4);
+    }
+    sm->abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if constexpr (QT == ARTLITE_IQ4_NL) {
+    constexpr int8_t v[16] = {-127, -104, -83, -65, -49, -35, -22, -10, 1, 13, 25, 38, 53, 69, 89, 113};
+    if (threadIdx.x < 256)
+      table[threadIdx.x] = Num<__half>::pack((float)v[threadIdx.x & 15], (float)v[threadIdx.x >> 4]);
+  }
+  if (warp == 0) tmem_alloc_pair(&sm->tmem_base);
+  tc::fence_before();
+  tc::cluster_sync();
+  tc::fence_after();
+  const uint32_t tmem = sm->tmem_base;
+
+  if (warp == 0 && lane == 0) {
+    // ---------------- the token rows (each CTA its 128)
+    int s = 0, ph = 0;
+    for (int id = pair; id < total; id += pairs) {
+      int m, n;
+      tile_at(p.order, id, &m, &n);
+      for (int ks = 0; ks < ksteps; ks++) {
+        if (!tc::wait(&sm->abort, &sm->empty[s], ph ^ 1, p.status, 40)) goto out;
+        if (crank == 0) tc::mbar_expect_tx(&sm->full_a[s], 2 * kStageBytes);
+        tc::tma_load_2d_pair(sA + s * kStageBytes, &p.map_x, tc::peer_addr(&sm->full_a[s], 0), ks * BK,
+                             m * TILE + HALF * (int)crank);
+        if (++s == S) s = 0, ph ^= 1;
+      }
+    }
+  } else if (warp == 1 && lane == 0 && crank == 0) {
+    // ---------------- the MMAs
+    int s = 0, ph = 0, acc = 0, aph = 0;
+    const uint32_t id_mma = tc::idesc_of(false, false, false, TILE, TILE);
+    for (int id = pair; id < total; id += pairs) {
+      if (!tc::wait_cluster(&sm->abort, &sm->tempty[acc], aph ^ 1, p.status, 41)) goto out;
+      tc::fence_after();
+      const uint32_t d = tmem + acc * TILE;
+      for (int ks = 0; ks < ksteps; ks++) {
+        if (!tc::wait_cluster(&sm->abort, &sm->full_a[s], ph, p.status, 42)) goto out;
+        if (!tc::wait_cluster(&sm->abort, &sm->full_b[s], ph, p.status, 43)) goto out;
+        tc::fence_after();
+        const uint64_t da = tc::sdesc(tc::smem_u32(sA + s * kStageBytes)), db = tc::sdesc(tc::smem_u32(sB + s * kStageBytes));
+#pragma unroll
+        for (int k = 0; k < BK / 16; k++) tc::mma_pair(d, da + 2 * k, db + 2 * k, id_mma, (ks | k) != 0);
+        tc::commit_pair(&sm->empty[s]);
+        if (++s == S) s = 0, ph ^= 1;
+      }
+      tc::commit_pair(&sm->tfull[acc]);
+      if (++acc == 2) acc = 0, aph ^= 1;
+    }
+  } else if (warp == 2 && lane == 0) {
+    // ---------------- the packed tiles: this CTA's 128 weight rows (8 row tiles), 256 values at a time
+    int r = 0, rph = 0;
+    for (int id = pair; id < total; id += pairs) {
+      int m, n;
+      tile_at(p.order, id, &m, &n);
+      const uint8_t* w = GATED ? p.w[crank] : p.w[0];
+      const int64_t mt0 = GATED ? 8 * (int64_t)n : 16 * (int64_t)n + 8 * crank;
+      // (past the matrix: its last rows again, whose products no output reads)
+      const int64_t mt = min64(mt0, p.row_tiles - 8);
+      for (int ch = 0; ch < chunks; ch++) {
+        if (!tc::wait(&sm->abort, &sm->raw_empty[r], rph ^ 1, p.status, 44)) goto out;
+        tc::mbar_expect_tx(&sm->raw_full[r], 8 * TB);
+        for (int i = 0; i < 8; i++)
+          bulk_copy(sR + (r * 8 + i) * TB, w + ((mt + i) * chunks + ch) * TB, TB, &sm->raw_full[r]);
+        if (++r == R) r = 0, rph ^= 1;
+      }
+    }
+  } else if (warp >= 8) {
+    // ---------------- the decoding: warp 8 + i turns row tile i of every stage into fp16 rows of B (K-major, 128-byte
+    // swizzle: 16-byte chunk c of row i at chunk c ^ (i & 7))
+    const int i = warp - 8, g = lane >> 2, t = lane & 3;
+    int s = 0, ph = 0, r = 0, rph = 0;
+    const uint32_t full_b0 = tc::peer_addr(&sm->full_b[0], 0);
+    for (int id = pair; id < total; id += pairs) {
+      for (int ch = 0; ch < chunks; ch++) {
+        if (!tc::wait(&sm->abort, &sm->raw_full[r], rph, p.status, 45)) goto out;
+        const uint8_t* tile = sR + (r * 8 + i) * TB;
+        const int units = min(kUnits, ksteps - kUnits * ch);
+        for (int u = 0; u < units; u++) {
+          const uint4 q = reinterpret_cast<const uint4*>(tile)[32 * u + lane];
+          Scales<QT> sc;
+          sc.load(tile, g, u);
+          // chunk[row][group]: eight values, words 2 j and 2 j + 1 of the lane's codes
+          uint4 c[2][2];
+#pragma unroll
+          for (int rr = 0; rr < 2; rr++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+              const uint32_t a = j ? q.z : q.x, b = j ? q.w : q.y;
+              c[rr][j] = make_uint4(decode_pair<QT>(a, rr, sc.d[rr][j], sc.m[rr][j], table),
+                                    decode_pair<QT>(a, 2 + rr, sc.d[rr][j], sc.m[rr][j], table),
+                                    decode_pair<QT>(b, rr, sc.d[rr][j], sc.m[rr][j], table),
+                                    decode_pair<QT>(b, 2 + rr, sc.d[rr][j], sc.m[rr][j], table));
+            }
+          if (!tc::wait(&sm->abort, &sm->empty[s], ph ^ 1, p.status, 46)) goto out;
+          uint8_t* row = sB + s * kStageBytes + (16 * i + g) * 128;
+          // (odd rows store their groups in the other order: eight lanes' 16-byte stores then fall in distinct banks)
+#pragma unroll
+          for (int rr = 0; rr < 2; rr++)
+#pragma unroll
+            for (int jj = 0; jj < 2; jj++) {
+              const int j = jj ^ (g & 1);
+              *reinterpret_cast<uint4*>(row + rr * 1024 + (((4 * j + t) ^ g) << 4)) = j ? c[rr][1] : c[rr][0];
+            }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            if (crank != 0) tc::arrive_cluster(full_b0 + s * (uint32_t)sizeof(uint64_t));
+            else tc::mbar_arrive(&sm->full_b[s]);
+          }
+          if (++s == S) s = 0, ph ^= 1;
+        }
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&sm->raw_empty[r]);
+        if (++r == R) r = 0, rph ^= 1;
+      }
+    }
+  } else if (warp >= 4) {
+    // ---------------- the epilogue: TMEM lanes 32 q .. + 31, a token row each
+    const int q = warp & 3;
+    int acc = 0, aph = 0;
+    const uint32_t tempty0 = tc::peer_addr(&sm->tempty[0], 0);
+    for (int id = pair; id < total; id += pairs) {
+      int m, n;
+      tile_at(p.order, id, &m, &n);
+      if (!tc::wait(&sm->abort, &sm->tfull[acc], aph, p.status, 47)) goto out;
+      tc::fence_after();
+      const uint32_t col0 = tmem + ((uint32_t)(32 * q) << 16) + acc * TILE;
+      const int tok = m * TILE + HALF * (int)crank + 32 * q + lane;
+      const bool live = tok < p.T;
+      const int e = live && p.row_exp ? p.row_exp[tok] : 0;
+      // 2^(row_exp - w_exp) in two factors (the exponents' sum may exceed one float's range)
+      const int e0 = e - p.w_exp0, e1 = e - p.w_exp1;
+      const float a0 = pow2(e0 / 2), a1 = pow2(e0 - e0 / 2);
+      const float b0 = pow2(e1 / 2), b1 = pow2(e1 - e1 / 2);
+      T* row = static_cast<T*>(p.y) + (int64_t)tok * p.ldy;
+      constexpr int kCols = GATED ? HALF : TILE;
+      for (int c = 0; c < kCols; c += 32) {
+        const int f = n * kCols + c;
+        uint32_t v[32];
+        float o[32];
+        tc::tmem_ld32(col0 + c, v);
+        if constexpr (GATED) {
+          uint32_t w[32];
+          tc::tmem_ld32(col0 + HALF + c, w);
+          tc::tmem_wait32(v);
+          tc::tmem_wait32(w);
+#pragma unroll
+          for (int j = 0; j < 32; j++)
+            o[j] = act_of<false>(p.act, __uint_as_float(v[j]) * a0 * a1) * (__uint_as_float(w[j]) * b0 * b1);
+        } else {
+          tc::tmem_wait32(v);
+#pragma unroll
+          for (int j = 0; j < 32; j++) o[j] = __uint_as_float(v[j]) * a0 * a1;
+        }
+        if (live) store32<T>(row + f, o, p.N - f, p.vec_y);
+      }
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (crank != 0) tc::arrive_cluster(tempty0 + acc * (uint32_t)sizeof(uint64_t));
+        else tc::mbar_arrive(&sm->tempty[acc]);
+      }
+      if (++acc == 2) acc = 0, aph ^= 1;
+    }
+  }
+out:
+  __syncwarp();
+  __syncthreads();
+  if (*(volatile int*)&sm->abort && threadIdx.x == 0) {  // let issued copies and MMAs land before TMEM is freed
+    const long long t0 = clock64();
+    while (clock64() - t0 < 20000000LL) {
+    }
+  }
+  tc::cluster_sync();  // (the leader's MMAs read the peer's shared memory until here)
+  if (warp == 0) {
+    tc::fence_after();
+    tmem_free_pair(tmem);
+  }
+}
+
+template <int QT, class T, bool GATED>
+int go(const Params& p, cudaStream_t st) {
+  int dev, sms;
+  AL_CUDA(cudaGetDevice(&dev));
+  AL_TRY(sm_count(dev, &sms));
+  const int total = p.order.tm * p.order.tn;
+  return launch_pairs(linear_gemm<QT, T, GATED>, p, total < sms / 2 ? total : sms / 2, kThreads, smem_bytes<QT>(), st);
+}
+template <int QT>
+int go_of(const Params& p, bool gated, bool bf16, cudaStream_t st) {
+  if (gated) return bf16 ? go<QT, __nv_bfloat16, true>(p, st) : go<QT, __half, true>(p, st);
+  return bf16 ? go<QT, __nv_bfloat16, false>(p, st) : go<QT, __half, false>(p, st);
+}
+
+}  // namespace
+
+namespace dg {
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+int make_operand_map(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int64_t ld, int box_x, int box_y) {
+  static const EncodeTiled enc = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                   q == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<EncodeTiled>(p)
+               : nullptr;
+  }();
+  AL_CHECK(enc, ARTLITE_ECUDA, "dense gemm: cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(ld * 2)};
+  const cuuint32_t box[2] = {(cuuint32_t)box_x, (cuuint32_t)box_y};
+  const cuuint32_t estr[2] = {1, 1};
+  // (16-bit words either way: a copy does not look at the type, and the fill is zero bits)
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  AL_CHECK(r == CUDA_SUCCESS, ARTLITE_ECUDA, "dense gemm: cuTensorMapEncodeTiled failed (%d): %lld x %lld, %lld apart",
+           (int)r, (long long)cols, (long long)rows, (long long)ld);
+  return ARTLITE_OK;
+}
+
+}  // namespace dg
+
+int launch_linear_gemm(const LinearGemmArgs& a, cudaStream_t st) {
+  Params p{};
+  AL_TRY(make_operand_map(&p.map_x, a.x, a.K, a.T, a.ldx, BK, HALF));
+  p.w[0] = a.w0;
+  p.w[1] = a.gated ? a.w1 : a.w0;
+  p.row_tiles = cdiv(a.N, kTileRows * kPadTiles) * kPadTiles;
+  p.y = a.y;
+  p.ldy = a.ldy;
+  p.row_exp = a.row_exp;
+  p.w_exp0 = a.w_exp0;
+  p.w_exp1 = a.w_exp1;
+  p.T = (int)a.T;
+  p.K = a.K;
+  p.N = a.N;
+  p.act = a.act;
+  p.vec_y = ((uintptr_t)a.y % 16) == 0 && a.ldy % 8 == 0;
+  p.order.tm = (int)cdiv(a.T, TILE);
+  p.order.tn = (int)cdiv(a.N, a.gated ? HALF : TILE);
+  p.status = a.status;
+  AL_CHECK((int64_t)p.order.tm * p.order.tn < (1ll << 31), ARTLITE_EUNSUPPORTED, "linear: T %lld by %d rows", (long long)a.T, a.N);
+  const bool bf16 = a.out_dtype == ARTLITE_BF16;
+  switch (a.qtype) {
+    case ARTLITE_Q4_0: return go_of<ARTLITE_Q4_0>(p, a.gated, bf16, st);
+    case ARTLITE_Q4_1: return go_of<ARTLITE_Q4_1>(p, a.gated, bf16, st);
+    case ARTLITE_Q4_K: return go_of<ARTLITE_Q4_K>(p, a.gated, bf16, st);
+    default: return go_of<ARTLITE_IQ4_NL>(p, a.gated, bf16, st);
+  }
+}
+
+}  // namespace artlite

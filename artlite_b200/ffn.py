@@ -1,0 +1,44 @@
+"""The gated feed-forward over plain bf16 / f16 matrices, forward and backward (``artlite_gated_ffn``,
+``artlite_gated_ffn_backward``, include/artlite_moe.h), on the caller's device buffers: addresses, or objects with
+``data_ptr()``. For 4-bit GGUF matrices: ``artlite_b200.linear.QuantLinear`` with ``up``."""
+
+import ctypes
+
+from ._lib import QTYPES, Error, check, lib
+from .linear import ACTIVATIONS
+from .moe.block import _ptr
+
+DTYPES = {"f16": "F16", "bf16": "BF16"}
+
+
+def _codes(dtype: str, activation: str) -> tuple[int, int]:
+    if dtype not in DTYPES or activation not in ACTIVATIONS:
+        raise Error(f"gated_ffn: type {dtype}, activation {activation}")
+    return QTYPES[DTYPES[dtype]], ACTIVATIONS[activation]
+
+
+def gated_ffn(x, w_gate, w_up, h, *, T: int, n_in: int, n_ffn: int, dtype: str = "bf16", activation: str = "silu",
+              gate=None, up=None, ldx: int | None = None, ldh: int | None = None, stream: int = 0) -> None:
+    """h (T, n_ffn) = act(x w_gate^T) * (x w_up^T) of x (T, n_in) and w_gate, w_up (n_ffn, n_in); ``gate``, ``up`` (T,
+    n_ffn) fp32: the two products, kept for ``gated_ffn_backward``. ``ldx``, ``ldh``: values between rows."""
+    dt, act = _codes(dtype, activation)
+    check(lib().artlite_gated_ffn(dt, act, _ptr(x), n_in if ldx is None else ldx, _ptr(w_gate), _ptr(w_up), _ptr(h),
+                                  n_ffn if ldh is None else ldh, _ptr(gate), _ptr(up), T, n_in, n_ffn,
+                                  ctypes.c_void_p(stream or None)))
+
+
+def gated_ffn_work_bytes(T: int, n_ffn: int) -> int:
+    """Bytes of ``gated_ffn_backward``'s ``work`` buffer."""
+    return lib().artlite_gated_ffn_work_bytes(T, n_ffn)
+
+
+def gated_ffn_backward(dh, x, w_gate, w_up, gate, up, work, *, T: int, n_in: int, n_ffn: int, dtype: str = "bf16",
+                       activation: str = "silu", dx=None, dw_gate=None, dw_up=None, lddh: int | None = None,
+                       ldx: int | None = None, lddx: int | None = None, stream: int = 0) -> None:
+    """The gradients of ``gated_ffn`` from dh (T, n_ffn) and the kept ``gate`` and ``up``: ``dx`` (T, n_in), ``dw_gate``
+    and ``dw_up`` (n_ffn, n_in), overwritten; None: not computed."""
+    dt, act = _codes(dtype, activation)
+    check(lib().artlite_gated_ffn_backward(dt, act, _ptr(dh), n_ffn if lddh is None else lddh, _ptr(x),
+                                           n_in if ldx is None else ldx, _ptr(w_gate), _ptr(w_up), _ptr(gate), _ptr(up),
+                                           _ptr(work), _ptr(dx), n_in if lddx is None else lddx, _ptr(dw_gate),
+                                           _ptr(dw_up), T, n_in, n_ffn, ctypes.c_void_p(stream or None)))

@@ -1,0 +1,67 @@
+"""Products with a 4-bit GGUF matrix outside an expert: ``QuantLinear`` (``artlite_linear_*``, include/artlite_moe.h).
+
+For a model's attention projections, its dense layers and its head, beside the block's experts: y = x W^T, or with a
+second matrix ``up`` the gated pair act(x W^T) * (x up^T). Host side: NumPy + ctypes."""
+
+import ctypes
+
+import numpy as np
+
+from ._lib import QTYPES, Error, LinearDesc, check, lib
+from .moe.block import _ptr
+
+ACTIVATIONS = {"silu": 0, "gelu": 1}
+ACT_DTYPES = {"f32": "F32", "f16": "F16", "bf16": "BF16"}
+
+
+class QuantLinear:
+    """A 4-bit GGUF matrix on one CUDA device: ``w`` (and ``up``) its raw rows (n_out rows of n_in values; Q4_0, Q4_1,
+    Q4_K or IQ4_NL), a numpy array or a device pointer, read before the constructor returns.
+
+    ``act_dtype``: "f32", "f16" or "bf16" (numpy: uint16 bit patterns) for x and y; ``activation``: "silu" or "gelu" (the
+    tanh form), used with ``up``."""
+
+    def __init__(self, w, *, n_in: int, n_out: int, qtype: str, act_dtype: str = "bf16", up=None,
+                 activation: str = "silu", device: int = -1):
+        if qtype not in QTYPES or act_dtype not in ACT_DTYPES or activation not in ACTIVATIONS:
+            raise Error(f"linear: type {qtype}, activation type {act_dtype}, activation {activation}")
+        self._h = None
+        self.n_in, self.n_out, self.act = n_in, n_out, act_dtype
+        keep = [np.ascontiguousarray(a) if isinstance(a, np.ndarray) else a for a in (w, up)]
+        d = LinearDesc(n_in=n_in, n_out=n_out, qtype=QTYPES[qtype], act_dtype=QTYPES[ACT_DTYPES[act_dtype]],
+                       activation=ACTIVATIONS[activation], device=device)
+        h = ctypes.c_void_p()
+        check(lib().artlite_linear_create(ctypes.byref(d), _ptr(keep[0]), _ptr(keep[1]), ctypes.byref(h)))
+        self._h = h
+
+    @property
+    def np_dtype(self):
+        return {"f32": np.float32, "f16": np.float16, "bf16": np.uint16}[self.act]
+
+    def forward(self, x: np.ndarray, out: np.ndarray | None = None) -> np.ndarray:
+        """y (T, n_out) of x (T, n_in) (host arrays: the call returns when y is back)."""
+        x = np.ascontiguousarray(x, self.np_dtype)
+        if x.ndim != 2 or x.shape[1] != self.n_in:
+            raise Error(f"linear: x has shape {x.shape}, n_in is {self.n_in}")
+        y = out if out is not None else np.empty((x.shape[0], self.n_out), self.np_dtype)
+        if y.shape != (x.shape[0], self.n_out) or y.dtype != self.np_dtype or not y.flags.c_contiguous:
+            raise Error(f"linear: out is {y.dtype} of shape {y.shape}")
+        self.forward_ptr(x, y, x.shape[0])
+        return y
+
+    def forward_ptr(self, x, y, T: int, *, ldx: int | None = None, ldy: int | None = None, stream: int = 0) -> None:
+        """The product on device buffers (addresses, or objects with ``data_ptr()``): T rows of x ``ldx`` values apart
+        (default n_in) and of y ``ldy`` apart (default n_out); enqueued on ``stream`` (0: the device's default)."""
+        check(lib().artlite_linear_forward(self._h, _ptr(x), self.n_in if ldx is None else ldx, _ptr(y),
+                                           self.n_out if ldy is None else ldy, T, ctypes.c_void_p(stream or None)))
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            lib().artlite_linear_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass

@@ -222,6 +222,70 @@ int64_t artlite_moe_launch_count(void);
 
 int artlite_moe_destroy(artlite_moe* h);
 
+/* ---------------------------------------------------------------- dense products beside the block
+ * The products of a model's layers that are not experts (no counterpart in the reference's operator API; its models run
+ * them as fused NPU operators, src/artlite/gemm and src/artlite/decode). All of them are enqueued on `stream` (a
+ * cudaStream_t of the buffers' device; NULL: that device's default stream) and return at once; they may be captured into
+ * a graph; the buffers' device need not be the current one. A bounded device wait that ran out is reported as
+ * ARTLITE_ETIMEOUT by the next of these calls on the device. Outputs must not overlap inputs. */
+
+/* activations of the gated pair */
+#define ARTLITE_ACT_SILU 0 /* z / (1 + e^-z) */
+#define ARTLITE_ACT_GELU 1 /* 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
+
+typedef struct artlite_linear artlite_linear;
+
+typedef struct {
+  int32_t n_in;       /* values a row of x and of the matrix (a multiple of the type's block: 32, Q4_K 256) */
+  int32_t n_out;      /* rows of the matrix, any number */
+  int32_t qtype;      /* ARTLITE_Q4_0, ARTLITE_Q4_1, ARTLITE_Q4_K or ARTLITE_IQ4_NL */
+  int32_t act_dtype;  /* x and y: ARTLITE_F32, ARTLITE_F16 or ARTLITE_BF16 */
+  int32_t activation; /* with w_up: ARTLITE_ACT_*; otherwise unused */
+  int32_t device;     /* CUDA device ordinal (-1: the current one) */
+} artlite_linear_desc;
+
+/*
+ * A 4-bit GGUF matrix for artlite_linear_forward: w the raw rows (n_out rows of n_in values), w_up NULL, or a second
+ * matrix of the same shape and type for the gated pair (a dense layer's ffn_gate and ffn_up). Host or device memory, read
+ * before the call returns and laid out for the kernels in as many bytes (rows padded to 128, values to 256).
+ */
+int artlite_linear_create(const artlite_linear_desc* desc, const void* w, const void* w_up, artlite_linear** out);
+
+/*
+ * y (T rows, ldy values apart) = x (T rows, ldx values apart) . w^T, or with w_up act(x . w^T) * (x . w_up^T). Sums in
+ * fp32. Up to 32 tokens, and any number of fp32 or unaligned ones: the products are exact and only the sums and the
+ * result round. Above (16-bit x with 16-byte aligned rows): each weight, and a bf16 x after scaling its row by a power of
+ * two, enters the tensor cores as fp16. An infinity or NaN in x makes that token's row of y NaN or infinite. x and y are
+ * both device memory of the handle's device, or both host memory (staged; the call returns when y is back). The handle
+ * keeps no state between calls: calls may overlap on any streams and in any captured graphs.
+ */
+int artlite_linear_forward(const artlite_linear* h, const void* x, int64_t ldx, void* y, int64_t ldy, int64_t T,
+                           void* stream);
+
+int artlite_linear_destroy(artlite_linear* h);
+
+/*
+ * The gated feed-forward over plain matrices: h (T x n_ffn, rows ldh apart) = act(x . w_gate^T) * (x . w_up^T), x (T x
+ * n_in, rows ldx apart), w_gate and w_up (n_ffn x n_in), all of dtype ARTLITE_BF16 or ARTLITE_F16; sums in fp32, h
+ * rounded once. gate, up (T x n_ffn fp32, both or neither): the products, kept for the backward pass. Device memory of
+ * one device, 16-byte aligned; n_in, n_ffn and the row distances multiples of 8.
+ */
+int artlite_gated_ffn(int dtype, int activation, const void* x, int64_t ldx, const void* w_gate, const void* w_up, void* h,
+                      int64_t ldh, float* gate, float* up, int64_t T, int n_in, int n_ffn, void* stream);
+
+/* Bytes of `work` for a backward pass. */
+int64_t artlite_gated_ffn_work_bytes(int64_t T, int n_ffn);
+
+/*
+ * Its backward pass, from dh (T x n_ffn, rows lddh apart) and the forward's gate and up: dg = dh up act'(gate), du = dh
+ * act(gate) (rounded to dtype into work), dx (T x n_in, rows lddx apart; may be NULL) = dg . w_gate + du . w_up, dw_gate =
+ * dg^T . x and dw_up = du^T . x (n_ffn x n_in; both or neither may be NULL), overwritten. Sums in fp32, in an order that
+ * does not depend on scheduling.
+ */
+int artlite_gated_ffn_backward(int dtype, int activation, const void* dh, int64_t lddh, const void* x, int64_t ldx,
+                               const void* w_gate, const void* w_up, const float* gate, const float* up, void* work, void* dx,
+                               int64_t lddx, void* dw_gate, void* dw_up, int64_t T, int n_in, int n_ffn, void* stream);
+
 /* ---------------------------------------------------------------- expert parallelism (ep_world > 1)
  * The reference runs on one NPU and has no counterpart (its closest analogue is the 8-column deal of moe_plan,
  * moe_host.cpp:216-234, an intra-device split). One process per GPU; rank r of W owns experts [r E / W, (r + 1) E / W)

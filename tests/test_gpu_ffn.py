@@ -1,0 +1,229 @@
+"""``gated_ffn`` and its backward pass against the formulas in 64 bits, and the gradients against differences.
+
+Tolerances. Products of 16-bit values are exact in fp32; a sum of n of them is off by at most n 2^-23 of its magnitudes'
+sum. h adds half a step. dg and du are rounded to 16 bits before the gradients' products: half a step of each term's
+magnitude, then the sums, then half a step of the result; over many outputs the roundings average, so the 2-norm is held
+to one step of the result's besides."""
+
+import numpy as np
+import pytest
+
+from tests.dense_helpers import EPS, act, slope, torch_dtype
+
+pytestmark = pytest.mark.gpu
+
+
+def inputs(seed, dtype, T, H, F, ldx=None):
+    import torch
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(seed)
+    dt = torch_dtype(dtype)
+
+    def n(*s, std=1.0):
+        return (torch.randn(*s, generator=gen, device="cuda") * std).to(dt)
+
+    x = n(T, ldx or H)
+    return x[:, :H], n(F, H, std=H ** -0.5), n(F, H, std=H ** -0.5), n(T, F, std=0.3)
+
+
+def forward64(x, wg, wu, activation):
+    g, u = x.double() @ wg.double().T, x.double() @ wu.double().T
+    return g, u, act(activation, g) * u
+
+
+def run_forward(x, wg, wu, activation, dtype, keep=True, ldh=None, stream=0):
+    import torch
+    from artlite_b200 import ffn
+    T, H = x.shape
+    F = wg.shape[0]
+    h = torch.full((T + 1, ldh or F), 3.0, dtype=x.dtype, device="cuda")
+    g, u = (torch.full((T + 1, F), 3.0, device="cuda") for _ in "gu") if keep else (None, None)
+    ffn.gated_ffn(x, wg, wu, h, T=T, n_in=H, n_ffn=F, dtype=dtype, activation=activation, gate=g, up=u,
+                  ldx=x.stride(0) if T > 1 else None, ldh=ldh, stream=stream)
+    return h, g, u
+
+
+def run_backward(dh, x, wg, wu, g, u, activation, dtype, stream=0, dx=True, dw=True):
+    import torch
+    from artlite_b200 import ffn
+    T, H = x.shape
+    F = wg.shape[0]
+    work = torch.empty(ffn.gated_ffn_work_bytes(T, F), dtype=torch.uint8, device="cuda")
+    out = [torch.full((T + 1, H), 3.0, dtype=x.dtype, device="cuda") if dx else None] + [
+        torch.full((F + 1, H), 3.0, dtype=x.dtype, device="cuda") if dw else None for _ in "gu"]
+    ffn.gated_ffn_backward(dh, x, wg, wu, g, u, work, T=T, n_in=H, n_ffn=F, dtype=dtype, activation=activation,
+                           dx=out[0], dw_gate=out[1], dw_up=out[2], ldx=x.stride(0) if T > 1 else None, stream=stream)
+    return out
+
+
+SHAPES = [(1, 64, 32), (2, 8, 8), (7, 136, 72), (8, 512, 96), (9, 200, 264), (16, 1032, 40), (31, 72, 130 * 8), (32, 256, 128),
+          (33, 264, 72), (64, 512, 128), (100, 8, 8), (129, 1032, 200), (256, 128, 256), (300, 328, 520), (513, 640, 264)]
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T,H,F", SHAPES)
+def test_forward(T, H, F, dtype, activation):
+    import torch
+    x, wg, wu, _ = inputs(T + H + F, dtype, T, H, F, ldx=H + 8)
+    h, g, u = run_forward(x, wg, wu, activation, dtype, ldh=F + 16)
+    g64, u64, want = forward64(x, wg, wu, activation)
+    dg = (H + 16) * 2.0 ** -23 * (x.double().abs() @ wg.double().abs().T)
+    du = (H + 16) * 2.0 ** -23 * (x.double().abs() @ wu.double().abs().T)
+    assert ((g[:T].double() - g64).abs() <= dg).all() and ((u[:T].double() - u64).abs() <= du).all()
+    tol = (1.13 * dg * u64.abs() + act(activation, g64).abs() * du + 1.13 * dg * du
+           + (EPS[dtype] / 2 * 1.01 + 2.0 ** -17) * want.abs() + 2.0 ** -22 * (dtype == "f16") + 1e-30)
+    err = (h[:T, :F].double() - want).abs()
+    assert (err <= tol).all(), f"max excess {(err - tol).max()}"
+    assert (h[T:] == 3).all() and (h[:, F:] == 3).all() and (g[T:] == 3).all() and (u[T:] == 3).all()
+    h2, _, _ = run_forward(x, wg, wu, activation, dtype, keep=False)
+    assert torch.equal(h2[:T], h[:T, :F])  # (with or without the kept values, and on a second run)
+
+
+def check_grad(got, want, terms, eps, what):
+    """terms: the sum of the products' magnitudes; its half steps, its fp32 sums and the result's half step."""
+    err = (got.double() - want).abs()
+    tol = terms * (eps / 2 * 1.02 + 2.0 ** -15) + eps / 2 * 1.01 * want.abs() + (2.0 ** -24 if eps == EPS["f16"] else 0) + 1e-30
+    assert (err <= tol).all(), f"{what}: max excess {(err - tol).max()}"
+    rms = err.norm() / want.norm()
+    assert rms <= eps, f"{what}: 2-norm {rms}"
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T,H,F", SHAPES)
+def test_backward(T, H, F, dtype, activation):
+    import torch
+    x, wg, wu, dh = inputs(T + H + F + 1, dtype, T, H, F, ldx=H + 8)
+    _, g, u = run_forward(x, wg, wu, activation, dtype)
+    dx, dwg, dwu = run_backward(dh, x, wg, wu, g, u, activation, dtype)
+    g64, u64, _ = forward64(x, wg, wu, activation)
+    dg, du = dh.double() * u64 * slope(activation, g64), dh.double() * act(activation, g64)
+    X, G, U = x.double(), wg.double(), wu.double()
+    eps = EPS[dtype]
+    # (fp16's subnormals: dg, du below 2^-14 are off by up to 2^-25 each)
+    tiny = 2.0 ** -25 if dtype == "f16" else 0.0
+    check_grad(dx[:T], dg @ G + du @ U, (dg.abs() + tiny * 2 / eps) @ G.abs() + (du.abs() + tiny * 2 / eps) @ U.abs(), eps, "dx")
+    check_grad(dwg[:F], dg.T @ X, (dg.abs() + tiny * 2 / eps).T @ X.abs(), eps, "dwg")
+    check_grad(dwu[:F], du.T @ X, (du.abs() + tiny * 2 / eps).T @ X.abs(), eps, "dwu")
+    assert all((o[n:] == 3).all() for o, n in ((dx, T), (dwg, F), (dwu, F)))
+    only_dx = run_backward(dh, x, wg, wu, g, u, activation, dtype, dw=False)
+    only_dw = run_backward(dh, x, wg, wu, g, u, activation, dtype, dx=False)
+    assert torch.equal(only_dx[0], dx) and torch.equal(only_dw[1], dwg) and torch.equal(only_dw[2], dwu)
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+def test_gradients_against_differences(activation):
+    """sum(h dh) moved along a random direction of x and of each matrix, in 64 bits, against the kernel's gradients. A
+    central difference with step 1e-4 of smooth functions is off by about 1e-8; the gradients by a step of bf16's."""
+    import torch
+    T, H, F = 70, 96, 64
+    x, wg, wu, dh = inputs(3, "bf16", T, H, F)
+    _, g, u = run_forward(x, wg, wu, activation, "bf16")
+    grads = run_backward(dh, x, wg, wu, g, u, activation, "bf16")
+    base = [x.double(), wg.double(), wu.double()]
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(4)
+    for i, n in enumerate((T, F, F)):
+        grad = grads[i][:n].double()
+        # along the gradient plus noise of its size, so that the slope is far from zero
+        v = grad + torch.randn(grad.shape, generator=gen, device="cuda", dtype=torch.float64) * grad.std()
+        v /= v.norm()
+        f = []
+        for s in (1e-4, -1e-4):
+            p = list(base)
+            p[i] = p[i] + s * v
+            f.append((forward64(*p, activation)[2] * dh.double()).sum())
+        diff, got = (f[0] - f[1]) / 2e-4, (grad * v).sum()
+        assert abs(diff - got) <= EPS["bf16"] * grad.norm(), (i, diff, got)
+
+
+def test_large_arguments():
+    """Gate values far out on both sides: the activation's ends, and slopes of 0 and 1."""
+    import torch
+    T, H, F = 40, 64, 64
+    for activation in ("silu", "gelu"):
+        x, wg, wu, dh = inputs(5, "bf16", T, H, F)
+        x = x * 64
+        _, g, u = run_forward(x, wg, wu, activation, "bf16")
+        dx, dwg, dwu = run_backward(dh, x, wg, wu, g, u, activation, "bf16")
+        assert all(torch.isfinite(t).all() for t in (dx, dwg, dwu))
+        g64, u64, _ = forward64(x, wg, wu, activation)
+        dg, du = dh.double() * u64 * slope(activation, g64), dh.double() * act(activation, g64)
+        check_grad(dwg[:F], dg.T @ x.double(), dg.abs().T @ x.double().abs(), EPS["bf16"], "dwg")
+        check_grad(dwu[:F], du.T @ x.double(), du.abs().T @ x.double().abs(), EPS["bf16"], "dwu")
+
+
+@pytest.mark.parametrize("T", [3, 40])
+def test_a_token_with_nan_leaves_the_others(T):
+    import torch
+    x, wg, wu, _ = inputs(6, "bf16", T, 128, 72)
+    x = x.contiguous()
+    want, _, _ = run_forward(x, wg, wu, "silu", "bf16")
+    x[1, 7] = float("nan")
+    got, _, _ = run_forward(x, wg, wu, "silu", "bf16")
+    assert torch.isnan(got[1]).all()
+    keep = [t for t in range(T + 1) if t != 1]
+    assert torch.equal(got[keep], want[keep])
+
+
+def test_no_tokens():
+    import torch
+    from artlite_b200 import ffn
+    w = torch.ones(16, 8, dtype=torch.bfloat16, device="cuda")
+    dw = [torch.full((16, 8), 5.0, dtype=torch.bfloat16, device="cuda") for _ in "gu"]
+    ffn.gated_ffn(None, w, w, None, T=0, n_in=8, n_ffn=16)
+    ffn.gated_ffn_backward(None, None, w, w, None, None, None, T=0, n_in=8, n_ffn=16, dw_gate=dw[0], dw_up=dw[1])
+    torch.cuda.synchronize()
+    assert all((d == 0).all() for d in dw)
+
+
+def test_a_training_step_captured_and_on_two_streams():
+    """Two training steps at once on two streams, then as two captured graphs replayed together: the same gradients."""
+    import torch
+    T, H, F = 150, 256, 136
+    sets = [inputs(s, "bf16", T, H, F) for s in (7, 8)]
+    want = []
+    for x, wg, wu, dh in sets:
+        h, g, u = run_forward(x, wg, wu, "silu", "bf16")
+        want.append([h] + run_backward(dh, x, wg, wu, g, u, "silu", "bf16"))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for st, (x, wg, wu, dh) in zip(streams, sets):
+        with torch.cuda.stream(st):
+            h, g, u = run_forward(x, wg, wu, "silu", "bf16", stream=st.cuda_stream)
+            got.append([h] + run_backward(dh, x, wg, wu, g, u, "silu", "bf16", stream=st.cuda_stream))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for w, o in zip(want, got) for a, b in zip(w, o))
+    graphs, outs = [], []
+    for x, wg, wu, dh in sets:
+        g_ = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g_):
+            s = torch.cuda.current_stream().cuda_stream
+            h, g, u = run_forward(x, wg, wu, "silu", "bf16", stream=s)
+            outs.append([h] + run_backward(dh, x, wg, wu, g, u, "silu", "bf16", stream=s))
+        graphs.append(g_)
+    for _ in range(3):
+        for st, g_ in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g_.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for w, o in zip(want, outs) for a, b in zip(w, o))
+
+
+def test_refusals_on_device():
+    import torch
+    from artlite_b200 import Error, ffn
+    x, wg, wu, dh = inputs(9, "bf16", 4, 64, 32)
+    h = torch.empty(4, 32, dtype=torch.bfloat16, device="cuda")
+    kw = dict(T=4, n_in=64, n_ffn=32)
+    with pytest.raises(Error, match="x is not 16-byte aligned"):
+        ffn.gated_ffn(x.data_ptr() + 2, wg, wu, h, **kw)
+    with pytest.raises(Error, match="rows are 60 apart"):
+        ffn.gated_ffn(x, wg, wu, h, ldx=60, **kw)
+    with pytest.raises(Error, match="w_up is not device memory"):
+        ffn.gated_ffn(x, wg, np.zeros(4096, np.uint64), h, **kw)
+    with pytest.raises(Error, match="null array"):
+        ffn.gated_ffn_backward(dh, x, wg, wu, None, None, None, dx=x, **kw)
+    torch.cuda.synchronize()
