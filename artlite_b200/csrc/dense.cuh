@@ -88,20 +88,30 @@ struct Num<float> {
 //
 // A matrix of N rows of K values is held as tiles of 16 rows x 256 values (K padded to 256 with zero scales, the rows
 // to 128), tile after tile along a row group, every tile one block of bytes:
-//   codes   [unit u of 64 values][lane = 4 g + t][16 B]: of row g and row g + 8, the values 64 u + 32 j + 8 t .. + 7 of
-//           the unit's two 32-value groups j. Word s = 2 j + h of the 16 bytes holds both rows' values 32 j + 8 t + 4 h
-//           .. + 3 as the eight nibbles of one mma.sync m16n8k16 step's A fragment (a0 = row g's first pair, a1 = row
-//           g + 8's, a2, a3 the second pairs): pair i in nibbles i and i + 4, so that (w >> 4 i) & 0x000F000F is the
-//           pair (IQ4_NL: in byte i, a 256-entry table's index). The k order inside a group is free as long as x follows
-//           it: lane t's x is eight consecutive values, and a step's sum stays inside one group.
-//   scales  [lane = 4 g + t] unit t's: Q4_0 / IQ4_NL 8 B: fp16 d of row g's two 32-value groups, then of row g + 8's;
-//           Q4_1 16 B: those and the same of m; Q4_K 8 B: for row g, then for row g + 8, a word of sc | mn << 6 of both
-//           groups in 24 bits and byte t of (d | dmin << 16) above.
+//   codes   [unit u of 64 values][lane = 4 g + t][16 B]: word 2 j + r holds values 8 t .. 8 t + 7 of the unit's 32-value
+//           group j of row g + 8 r: value 2 i in nibble i, value 2 i + 1 in nibble i + 4, so that (w >> 4 i) & 0x000F000F
+//           is pair i, an mma.sync m16n8k16 fragment's register once it is made floating-point, and the word's bytes are
+//           an m16n8k32 integer fragment's as they are (IQ4_NL: pair i in byte i, a 256-entry table's index). The k order
+//           inside a group is free as long as x follows it.
+//   scales  Q4_0 / IQ4_NL [g][u][j] 4 B: fp16 d of row g and of row g + 8; Q4_1 [g][u][j] 8 B: that and the same of m;
+//           Q4_K [g][j] 16 B: words 0 - 2 hold the four units' fields, 24 bits each (sc | mn << 6 of row g, then of row
+//           g + 8; unit 3's in the three top bytes), word 3 d | dmin << 16 of row g + 8 j.
 // The bytes of a tile are the raw blocks' (2304 for 4096 values of Q4_0, Q4_K, IQ4_NL; 2560 for Q4_1).
 constexpr int kTileRows = 16, kTileK = 256, kUnits = 4, kCodeBytes = 2048;
 constexpr int kPadTiles = 8;  // row tiles are padded to whole 128-row groups
 __host__ __device__ constexpr int scale_bytes(int qt) { return qt == ARTLITE_Q4_1 ? 512 : 256; }
 __host__ __device__ constexpr int tile_bytes(int qt) { return kCodeBytes + scale_bytes(qt); }
+
+// unit u's 24 bits of a Q4_K scale block
+__device__ __forceinline__ uint32_t k_fields(const uint4& v, int u) {
+  return u == 0   ? v.x
+         : u == 1 ? v.y
+         : u == 2 ? v.z
+                  : __byte_perm(__byte_perm(v.x, v.y, 0x0073), v.z, 0x0710);
+}
+// six bits of v from bit `at`, as the float 2^23 + field: a fused multiply-add by d with -2^23 d is then d times the
+// field exactly
+__device__ __forceinline__ float k_field(uint32_t v, int at) { return __uint_as_float(((v >> at) & 63u) | 0x4B000000u); }
 
 // ---------------------------------------------------------------- host side
 

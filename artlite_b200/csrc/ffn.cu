@@ -2,6 +2,7 @@
 // checks, the choice of kernel, and the backward pass's elementwise step. No state: every buffer is the caller's.
 #include <cuda_runtime.h>
 
+#include "dense_gemm.cuh"
 #include "ffn.cuh"
 #include "kernels.cuh"
 #include "small_batch.cuh"
@@ -55,11 +56,11 @@ int launch_gate_grad(const FfnArgs& a, cudaStream_t st) {
 // tokens up to which the small-batch kernel runs
 constexpr int64_t kSmallTokens = 32;
 
-int forward(const FfnArgs& a, cudaStream_t st) {
-  if (a.T > kSmallTokens) return launch_ffn_forward_gemm(a, st);
+int forward(const FfnArgs& a, int dev, cudaStream_t st) {
+  if (a.T > kSmallTokens || a.H > sb::kMaxK) return launch_ffn_forward_gemm(a, st);
   sb::Args s{};
-  s.w0 = a.wg;
-  s.w1 = a.wu;
+  AL_TRY(dg::make_operand_map(&s.map[0], a.wg, a.H, a.F, a.H, 64, kTileRows));
+  AL_TRY(dg::make_operand_map(&s.map[1], a.wu, a.H, a.F, a.H, 64, kTileRows));
   s.x = a.x;
   s.y = a.h;
   s.ldx = a.ldx;
@@ -68,10 +69,12 @@ int forward(const FfnArgs& a, cudaStream_t st) {
   s.K = a.H;
   s.N = a.F;
   s.act = a.act;
+  s.vec = 1;
   s.keep_g = a.g;
   s.keep_u = a.u;
-  if (a.dtype == ARTLITE_BF16) return sb::launch<sb::Plain<__nv_bfloat16>, __nv_bfloat16, true, true>(s, st);
-  return sb::launch<sb::Plain<__half>, __half, true, true>(s, st);
+  s.status = a.status;
+  if (a.dtype == ARTLITE_BF16) return sb::launch<sb::Plain<__nv_bfloat16>, __nv_bfloat16, true>(s, dev, st);
+  return sb::launch<sb::Plain<__half>, __half, true>(s, dev, st);
 }
 
 // the checks both passes share; *dev: the device of the buffers
@@ -140,7 +143,7 @@ int artlite_gated_ffn(int dtype, int activation, const void* x, int64_t ldx, con
   a.H = n_in;
   a.F = n_ffn;
   AL_TRY(dense_status(dev, &a.status));
-  return forward(a, static_cast<cudaStream_t>(stream));
+  return forward(a, dev, static_cast<cudaStream_t>(stream));
 }
 
 int artlite_gated_ffn_backward(int dtype, int activation, const void* dh, int64_t lddh, const void* x, int64_t ldx,

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <math.h>
 
+#include <algorithm>
 #include <memory>
 #include <mutex>
 #include <new>
@@ -120,7 +121,7 @@ __device__ __forceinline__ int code_at(int qt, const uint8_t* row, int k) {
   return i < 16 ? c & 15 : c >> 4;
 }
 
-__device__ __forceinline__ uint32_t half_bits(float v) { return __half_as_ushort(__float2half_rn(v)); }
+__device__ __forceinline__ uint32_t half_at(const uint8_t* p) { return p[0] | (uint32_t)p[1] << 8; }
 
 // the largest magnitude any scale, minimum or value of the matrix has, as fp32 bits (non-negative floats order as ints)
 __global__ void weight_bound_kernel(int qt, const uint8_t* raw, int64_t rb, int64_t N, int K, uint32_t* bound) {
@@ -147,9 +148,9 @@ __global__ void weight_bound_kernel(int qt, const uint8_t* raw, int64_t rb, int6
   if ((threadIdx.x & 31) == 0) atomicMax(bound, __float_as_uint(m));
 }
 
-// one warp a packed tile (dense.cuh); scale: 2^w_exp
+// one warp a packed tile (dense.cuh)
 __global__ void pack_kernel(int qt, const uint8_t* raw, int64_t rb, int64_t N, int K, int64_t row_tiles, int chunks,
-                            float scale, uint8_t* out) {
+                            uint8_t* out) {
   const int64_t tile = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (tile >= row_tiles * chunks) return;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -163,48 +164,48 @@ __global__ void pack_kernel(int qt, const uint8_t* raw, int64_t rb, int64_t N, i
   }
   for (int u = 0; u < kUnits; u++) {
     uint32_t w[4];
-    for (int s = 0; s < 4; s++) {
-      const int k = kTileK * ch + 64 * u + 32 * (s >> 1) + 8 * t + 4 * (s & 1);
+    for (int s = 0; s < 4; s++) {  // group s / 2 of row s % 2
+      const int k = kTileK * ch + 64 * u + 32 * (s >> 1) + 8 * t;
       uint32_t v = 0;
-      for (int i = 0; i < 4; i++) {  // pair i: row i & 1, values 2 (i >> 1) and + 1
-        for (int e = 0; e < 2; e++) {
-          const int kk = k + 2 * (i >> 1) + e;
-          const uint32_t c = row[i & 1] && kk < K ? (uint32_t)code_at(qt, row[i & 1], kk) : 0u;
-          v |= c << (qt == ARTLITE_IQ4_NL ? 8 * i + 4 * e : 4 * i + 16 * e);
-        }
+      for (int i = 0; i < 8; i++) {
+        const uint32_t c = row[s & 1] && k + i < K ? (uint32_t)code_at(qt, row[s & 1], k + i) : 0u;
+        v |= c << (qt == ARTLITE_IQ4_NL ? 4 * i : 4 * (i >> 1) + 16 * (i & 1));
       }
       w[s] = v;
     }
     reinterpret_cast<uint4*>(o)[32 * u + lane] = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  // lane 4 g + t: unit t's scales
-  uint32_t s[4] = {0, 0, 0, 0};
-  for (int r = 0; r < 2; r++) {
-    if (!row[r]) continue;
-    if (qt == ARTLITE_Q4_K) {
-      if (kTileK * ch >= K) continue;
+  if (qt == ARTLITE_Q4_K) {
+    if (t >= 2) return;
+    uint32_t f[4] = {0, 0, 0, 0}, dd = 0;  // (group 2 u + t of unit u)
+    for (int r = 0; r < 2; r++) {
+      if (!row[r]) continue;
       const uint8_t* b = row[r] + (int64_t)ch * 144;
-      uint32_t v = 0;
-      for (int j = 0; j < 2; j++) {
+      if (r == t) dd = half_at(b) | half_at(b + 2) << 16;
+      for (int u = 0; u < kUnits; u++) {
         int sc, mn;
-        k_scale_min(b, 2 * t + j, &sc, &mn);
-        v |= (uint32_t)(sc | mn << 6) << (12 * j);
-      }
-      const uint32_t dd = half_bits(f16_at(b) * scale) | half_bits(f16_at(b + 2) * scale) << 16;
-      s[r] = v | ((dd >> (8 * t)) & 0xFFu) << 24;
-    } else {
-      const int size = qt == ARTLITE_Q4_1 ? 20 : 18;
-      for (int j = 0; j < 2; j++) {
-        const int k = kTileK * ch + 64 * t + 32 * j;
-        if (k >= K) continue;
-        const uint8_t* b = row[r] + (int64_t)(k >> 5) * size;
-        s[r] |= half_bits(f16_at(b) * scale) << (16 * j);
-        if (qt == ARTLITE_Q4_1) s[2 + r] |= half_bits(f16_at(b + 2) * scale) << (16 * j);
+        k_scale_min(b, 2 * u + t, &sc, &mn);
+        f[u] |= (uint32_t)(sc | mn << 6) << (12 * r);
       }
     }
+    reinterpret_cast<uint4*>(o + kCodeBytes)[2 * g + t] =
+        make_uint4(f[0] | f[3] << 24, f[1] | ((f[3] >> 8) & 0xFFu) << 24, f[2] | (f[3] >> 16) << 24, dd);
+    return;
   }
-  if (qt == ARTLITE_Q4_1) reinterpret_cast<uint4*>(o + kCodeBytes)[lane] = make_uint4(s[0], s[1], s[2], s[3]);
-  else reinterpret_cast<uint2*>(o + kCodeBytes)[lane] = make_uint2(s[0], s[1]);
+  const int size = qt == ARTLITE_Q4_1 ? 20 : 18;
+  for (int j = 0; j < 2; j++) {  // unit t's groups
+    const int k = kTileK * ch + 64 * t + 32 * j;
+    uint32_t d = 0, m = 0;
+    for (int r = 0; r < 2; r++) {
+      if (!row[r] || k >= K) continue;
+      const uint8_t* b = row[r] + (int64_t)(k >> 5) * size;
+      d |= half_at(b) << (16 * r);
+      if (qt == ARTLITE_Q4_1) m |= half_at(b + 2) << (16 * r);
+    }
+    uint32_t* at = reinterpret_cast<uint32_t*>(o + kCodeBytes);
+    if (qt == ARTLITE_Q4_1) at[2 * (8 * g + 2 * t + j)] = d, at[2 * (8 * g + 2 * t + j) + 1] = m;
+    else at[8 * g + 2 * t + j] = d;
+  }
 }
 
 // x's rows as scaled fp16 (linear.cuh): a CTA a row
@@ -291,33 +292,33 @@ int pack(artlite_linear* h, int which, const void* raw) {
   AL_LAUNCHED();
   float m;
   AL_CUDA(cudaMemcpy(&m, bound.ptr, 4, cudaMemcpyDeviceToHost));
-  // the packed scales are the file's times 2^w_exp: the largest value below 2^15, so that the prompt kernel's fp16
-  // weights cannot overflow and only values 2^-29 below the largest lose bits
-  int e = 0;
-  if (m > 0.0f && isfinite(m)) e = 14 - ilogbf(m);
-  h->w_exp[which] = e;
+  // the prompt kernel multiplies the scales by 2^w_exp: the largest weight then lies below 2^15 in fp16, and only those
+  // 2^-29 below it lose bits (a matrix whose largest is under 2^-14 stays smaller than that)
+  if (m > 0.0f && isfinite(m)) h->w_exp[which] = std::min(std::max(14 - ilogbf(m), -14), 28);
   const int chunks = (int)cdiv(K, kTileK);
   const int64_t row_tiles = cdiv(N, kTileRows * kPadTiles) * kPadTiles;
   AL_TRY(h->w[which].reserve((size_t)(row_tiles * chunks * tile_bytes(qt))));
-  pack_kernel<<<(unsigned)cdiv(row_tiles * chunks, 8), 256>>>(qt, src, rb, N, K, row_tiles, chunks, ldexpf(1.0f, e),
+  pack_kernel<<<(unsigned)cdiv(row_tiles * chunks, 8), 256>>>(qt, src, rb, N, K, row_tiles, chunks,
                                                                 h->w[which].as<uint8_t>());
   AL_LAUNCHED();
   AL_CUDA(cudaDeviceSynchronize());
   return ARTLITE_OK;
 }
 
-template <int QT, class XT, bool VEC>
-int small(const sb::Args& a, bool gated, cudaStream_t st) {
-  return gated ? sb::launch<sb::Quant<QT>, XT, true, VEC>(a, st) : sb::launch<sb::Quant<QT>, XT, false, VEC>(a, st);
-}
-template <class XT, bool VEC>
-int small_of(int qt, const sb::Args& a, bool gated, cudaStream_t st) {
+template <class XT>
+int small_of(int qt, const sb::Args& a, bool gated, int dev, cudaStream_t st) {
   switch (qt) {
-    case ARTLITE_Q4_0: return small<ARTLITE_Q4_0, XT, VEC>(a, gated, st);
-    case ARTLITE_Q4_1: return small<ARTLITE_Q4_1, XT, VEC>(a, gated, st);
-    case ARTLITE_Q4_K: return small<ARTLITE_Q4_K, XT, VEC>(a, gated, st);
-    default: return small<ARTLITE_IQ4_NL, XT, VEC>(a, gated, st);
+#define AL_SB_CASE(QT) \
+  case QT: return gated ? sb::launch<sb::Quant<QT>, XT, true>(a, dev, st) : sb::launch<sb::Quant<QT>, XT, false>(a, dev, st);
+    AL_SB_CASE(ARTLITE_Q4_0)
+    AL_SB_CASE(ARTLITE_Q4_1)
+    AL_SB_CASE(ARTLITE_Q4_K)
+    AL_SB_CASE(ARTLITE_IQ4_NL)
+#undef AL_SB_CASE
+    default: break;
   }
+  set_error("linear: type %d", qt);
+  return ARTLITE_EUNSUPPORTED;
 }
 
 // tokens up to which the small-batch kernel runs
@@ -359,8 +360,8 @@ int run(const artlite_linear* h, const void* x, int64_t ldx, void* y, int64_t ld
     return rc != ARTLITE_OK ? rc : rf;
   }
   sb::Args a{};
-  a.w0 = h->w[0].ptr;
-  a.w1 = h->w[1].ptr;
+  a.w[0] = h->w[0].as<uint8_t>();
+  a.w[1] = h->w[1].as<uint8_t>();
   a.x = x;
   a.y = y;
   a.ldx = ldx;
@@ -369,14 +370,11 @@ int run(const artlite_linear* h, const void* x, int64_t ldx, void* y, int64_t ld
   a.K = d.n_in;
   a.N = d.n_out;
   a.act = d.activation;
-  a.scale0 = ldexpf(1.0f, -h->w_exp[0]);
-  a.scale1 = ldexpf(1.0f, -h->w_exp[1]);
-  if (d.act_dtype == ARTLITE_F32)
-    return vec ? small_of<float, true>(d.qtype, a, h->gated, st) : small_of<float, false>(d.qtype, a, h->gated, st);
-  if (d.act_dtype == ARTLITE_F16)
-    return vec ? small_of<__half, true>(d.qtype, a, h->gated, st) : small_of<__half, false>(d.qtype, a, h->gated, st);
-  return vec ? small_of<__nv_bfloat16, true>(d.qtype, a, h->gated, st)
-             : small_of<__nv_bfloat16, false>(d.qtype, a, h->gated, st);
+  a.vec = vec;
+  a.status = h->status;
+  if (d.act_dtype == ARTLITE_F32) return small_of<float>(d.qtype, a, h->gated, h->dev, st);
+  if (d.act_dtype == ARTLITE_F16) return small_of<__half>(d.qtype, a, h->gated, h->dev, st);
+  return small_of<__nv_bfloat16>(d.qtype, a, h->gated, h->dev, st);
 }
 
 }  // namespace
@@ -390,8 +388,9 @@ int artlite_linear_create(const artlite_linear_desc* desc, const void* w, const 
   const artlite_linear_desc& d = *desc;
   AL_CHECK(linear_type(d.qtype), ARTLITE_EUNSUPPORTED, "linear: GGUF type %s (Q4_0, Q4_1, Q4_K and IQ4_NL are read)",
            qtype_name(d.qtype));
-  AL_CHECK(d.n_in >= 1 && d.n_out >= 1 && d.n_in <= (1 << 24) && d.n_in % q_per(d.qtype) == 0, ARTLITE_EINVAL,
-           "linear: %d values a row, %d rows (rows are whole blocks of %d values)", d.n_in, d.n_out, q_per(d.qtype));
+  AL_CHECK(d.n_in >= 1 && d.n_out >= 1 && d.n_in <= sb::kMaxK && d.n_in % q_per(d.qtype) == 0, ARTLITE_EINVAL,
+           "linear: %d values a row, %d rows (rows are whole blocks of %d values, at most %d)", d.n_in, d.n_out,
+           q_per(d.qtype), sb::kMaxK);
   AL_CHECK(d.act_dtype == ARTLITE_F32 || d.act_dtype == ARTLITE_F16 || d.act_dtype == ARTLITE_BF16, ARTLITE_EINVAL,
            "linear: activation type %d", d.act_dtype);
   AL_CHECK(!w_up || d.activation == kActSilu || d.activation == kActGelu, ARTLITE_EINVAL, "linear: activation %d",

@@ -13,7 +13,7 @@ struct LinearGemmArgs {
   const uint16_t* x;      // fp16 rows, ldx apart (a multiple of 8), 16-byte aligned
   int64_t ldx;
   const int32_t* row_exp; // (may be null) row t of x holds the row's values times 2^-row_exp[t]
-  int w_exp0, w_exp1;     // the packed scales are the file's times 2^w_exp
+  int w_exp0, w_exp1;     // powers of two for the scales: 2^w_exp keeps the matrix inside fp16
   void* y;
   int64_t ldy;
   int out_dtype;          // ARTLITE_BF16 or ARTLITE_F16

@@ -10,8 +10,8 @@
 // The operands are fp16 for either activation type: a code times its group's scale rounds once to 11 significant bits
 // (bf16 would keep 8: a bf16 weight's rounding alone is as large as the output's, measured 0.0024 against 0.0017 of the
 // result's norm). bf16 x fits after a row's values are multiplied by a power of two (linear.cu half_rows_kernel); fp16's
-// range then loses only what is 2^-29 below a row's largest value. The packed scales carry a power of two too; the
-// epilogue undoes both.
+// range then loses only what is 2^-29 below a row's largest value. The scales are multiplied by a power of two
+// too; the epilogue undoes both.
 //
 // Warps: 0 the token rows' TMA, 1 the MMAs (the leader CTA's), 2 the packed tiles' copies, 3 idle, 4 - 7 the epilogue,
 // 8 - 15 the decoding.
@@ -71,44 +71,46 @@ __device__ __forceinline__ uint32_t u32(__half2 v) { return *reinterpret_cast<co
 template <int QT>
 struct Scales {
   __half2 d[2][2], m[2][2];
-  __device__ __forceinline__ void load(const uint8_t* tile, int g, int u) {
+  // f0 f1: the matrix's power of two, in two factors that fp16 holds
+  __device__ __forceinline__ void load(const uint8_t* tile, int g, int u, __half2 f0, __half2 f1) {
     const uint8_t* p = tile + kCodeBytes;
-    if constexpr (QT == ARTLITE_Q4_1) {
-      const uint4 v = reinterpret_cast<const uint4*>(p)[4 * g + u];
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    if constexpr (QT == ARTLITE_Q4_K) {
+      const uint4 v[2] = {reinterpret_cast<const uint4*>(p)[2 * g], reinterpret_cast<const uint4*>(p)[2 * g + 1]};
 #pragma unroll
       for (int r = 0; r < 2; r++) {
-        d[r][0] = __low2half2(h2(w[r])), d[r][1] = __high2half2(h2(w[r]));
-        m[r][0] = __low2half2(h2(w[2 + r])), m[r][1] = __high2half2(h2(w[2 + r]));
-      }
-    } else if constexpr (QT == ARTLITE_Q4_K) {
-      uint2 v[4];
-#pragma unroll
-      for (int t = 0; t < 4; t++) v[t] = reinterpret_cast<const uint2*>(p)[4 * g + t];
-      const uint2 mine = u == 0 ? v[0] : u == 1 ? v[1] : u == 2 ? v[2] : v[3];
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        const uint32_t dd = r ? (v[0].y >> 24) | (v[1].y >> 24) << 8 | (v[2].y >> 24) << 16 | (v[3].y & 0xFF000000u)
-                              : (v[0].x >> 24) | (v[1].x >> 24) << 8 | (v[2].x >> 24) << 16 | (v[3].x & 0xFF000000u);
-        const float2 f = __half22float2(h2(dd));
-        const uint32_t w = r ? mine.y : mine.x;
+        const float2 f = __half22float2(__hmul2(__hmul2(h2(v[r].w), f0), f1));
 #pragma unroll
         for (int j = 0; j < 2; j++) {
           // (the products of the file's fp16 and 6-bit scales round to fp16: 2^-12 of a weight, against the output's
           // 2^-9 in bf16)
-          d[r][j] = __float2half2_rn(f.x * (float)((w >> (12 * j)) & 63u));
-          m[r][j] = __float2half2_rn(-f.y * (float)((w >> (12 * j + 6)) & 63u));
+          const uint32_t w = k_fields(v[j], u);
+          d[r][j] = __float2half2_rn(fmaf(k_field(w, 12 * r), f.x, -8388608.0f * f.x));
+          m[r][j] = __float2half2_rn(-fmaf(k_field(w, 12 * r + 6), f.y, -8388608.0f * f.y));
         }
       }
     } else {
-      const uint2 v = reinterpret_cast<const uint2*>(p)[4 * g + u];
-      d[0][0] = __low2half2(h2(v.x)), d[0][1] = __high2half2(h2(v.x));
-      d[1][0] = __low2half2(h2(v.y)), d[1][1] = __high2half2(h2(v.y));
+      uint32_t w[2][2];  // [d, m][group]
+      if constexpr (QT == ARTLITE_Q4_1) {
+        const uint4 v = reinterpret_cast<const uint4*>(p)[4 * g + u];
+        w[0][0] = v.x, w[1][0] = v.y, w[0][1] = v.z, w[1][1] = v.w;
+      } else {
+        const uint2 v = reinterpret_cast<const uint2*>(p)[4 * g + u];
+        w[0][0] = v.x, w[0][1] = v.y;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const __half2 a = __hmul2(__hmul2(h2(w[0][j]), f0), f1);
+        d[0][j] = __low2half2(a), d[1][j] = __high2half2(a);
+        if constexpr (QT == ARTLITE_Q4_1) {
+          const __half2 b = __hmul2(__hmul2(h2(w[1][j]), f0), f1);
+          m[0][j] = __low2half2(b), m[1][j] = __high2half2(b);
+        }
+      }
     }
   }
 };
 
-// word w's pair i (row i & 1) with its group's scale: one rounding to fp16 from the exact code
+// word w's pair i with its group's scale: one rounding to fp16 from the exact code
 template <int QT>
 __device__ __forceinline__ uint32_t decode_pair(uint32_t w, int i, __half2 d, __half2 m, const uint32_t* table) {
   if constexpr (QT == ARTLITE_IQ4_NL) {
@@ -223,6 +225,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
     const int i = warp - 8, g = lane >> 2, t = lane & 3;
     int s = 0, ph = 0, r = 0, rph = 0;
     const uint32_t full_b0 = tc::peer_addr(&sm->full_b[0], 0);
+    const int we = GATED && crank ? p.w_exp1 : p.w_exp0;
+    const __half2 f0 = __float2half2_rn(pow2(we / 2)), f1 = __float2half2_rn(pow2(we - we / 2));
     for (int id = pair; id < total; id += pairs) {
       for (int ch = 0; ch < chunks; ch++) {
         if (!tc::wait(&sm->abort, &sm->raw_full[r], rph, p.status, 45)) goto out;
@@ -231,18 +235,18 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
         for (int u = 0; u < units; u++) {
           const uint4 q = reinterpret_cast<const uint4*>(tile)[32 * u + lane];
           Scales<QT> sc;
-          sc.load(tile, g, u);
-          // chunk[row][group]: eight values, words 2 j and 2 j + 1 of the lane's codes
+          sc.load(tile, g, u, f0, f1);
+          // chunk [row][group]: eight values, word 2 j + row of the lane's codes
           uint4 c[2][2];
 #pragma unroll
           for (int rr = 0; rr < 2; rr++)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-              const uint32_t a = j ? q.z : q.x, b = j ? q.w : q.y;
-              c[rr][j] = make_uint4(decode_pair<QT>(a, rr, sc.d[rr][j], sc.m[rr][j], table),
-                                    decode_pair<QT>(a, 2 + rr, sc.d[rr][j], sc.m[rr][j], table),
-                                    decode_pair<QT>(b, rr, sc.d[rr][j], sc.m[rr][j], table),
-                                    decode_pair<QT>(b, 2 + rr, sc.d[rr][j], sc.m[rr][j], table));
+              const uint32_t a = rr ? (j ? q.w : q.y) : (j ? q.z : q.x);
+              c[rr][j] = make_uint4(decode_pair<QT>(a, 0, sc.d[rr][j], sc.m[rr][j], table),
+                                    decode_pair<QT>(a, 1, sc.d[rr][j], sc.m[rr][j], table),
+                                    decode_pair<QT>(a, 2, sc.d[rr][j], sc.m[rr][j], table),
+                                    decode_pair<QT>(a, 3, sc.d[rr][j], sc.m[rr][j], table));
             }
           if (!tc::wait(&sm->abort, &sm->empty[s], ph ^ 1, p.status, 46)) goto out;
           uint8_t* row = sB + s * kStageBytes + (16 * i + g) * 128;

@@ -1,40 +1,55 @@
-// The small-batch product: y (T x N) = x (T x K) . W^T for a few tokens, W streamed once from HBM straight into
-// mma.sync fragments. With T <= 8 a token tile's 8 columns are the MMA's N, so every weight is read once for 8 tokens;
-// the bound is the weight bytes.
+// The small-batch product: y (T x N) = x (T x K) . W^T for a few tokens, W streamed once from HBM through shared memory
+// into mma.sync m16n8k16 fragments. Up to 8 tokens are the MMA's N (16 and 32 tokens: two and four of them), so every
+// weight is read and decoded once for all of them; the bound is the weight bytes.
 //
-// A CTA owns MT 16-row tiles (linear: 16 MT output rows; gated: tile 0 the gate rows and tile 1 the up rows of the same
-// 16 features) and 8 NT tokens; its 8 warps split K chunk by chunk (a chunk is 256 values of 4-bit weights, 64 of
-// 16-bit ones, 16 B a lane a load) and their partial sums meet in shared memory in a fixed order, so results do not
-// depend on scheduling. A lane's weight loads are 16 consecutive bytes of the fragment it feeds to the MMA: no shared
-// memory and no shuffles on the weights' way. The next chunk's weights are in flight while this one is multiplied.
-// x is read from L1 / L2 in the same k order (eight consecutive values a lane and 32-value group). fp32 x is cut into three bf16 planes whose
-// sum it is exactly (24 bits = 8 + 8 + 8), each multiplied into the same fp32 accumulator.
+// Work: a tile is 16 output rows, an item 256 (4-bit) or 64 (16-bit) of a tile's K values, about 2 KB that one bulk or TMA
+// copy brings. A cluster of c CTAs owns a range of tiles and each of its CTAs 1 / c of K; in a CTA, wk warps share a
+// tile's items and 16 / wk tiles run at a time. A warp has its own ring of D items in flight and its own barriers: no
+// warp waits for another until a batch of tiles is done, when the partial sums meet in shared memory (over the cluster
+// by distributed shared memory) in a fixed order, so results do not depend on scheduling. x lies in shared memory in
+// fragment order, fp32 x as three bf16 planes whose sum it is exactly (24 bits = 8 + 8 + 8), all of which multiply into
+// one fp32 accumulator. c, wk and D follow from the sizes (plan below).
 //
-// 4-bit weights: the codes become exact small integers in bf16 / fp16 (128 + q or 1024 + q by one logic operation, the
-// offset taken away exactly), their products with x are exact in fp32, a 32-value group's sum is multiplied by the
-// group's fp32 scale; the minimum term of Q4_1 / Q4_K is the group's sum of x (an MMA with ones) times the minimum. No
-// rounding but the fp32 sums' and the output's.
+// 4-bit weights: the codes become exact small integers in bf16 / fp16, their products with x are exact in fp32, and a
+// 32-value group's sum is multiplied by the group's fp32 scale. The minimum of Q4_1 / Q4_K times the group's sum of x is
+// one more term. One logic operation and one shift make 16 + q (bf16: 0x4180 | q << 3, fp16: 0x4C00 | q << 6); for
+// Q4_1 / Q4_K the 16 is taken away with the minimum's term, 16 scale times the sum of x (fp32 rounding of a value 17 / q
+// times the group's: 2^-20 of it at most, far under a 16-bit result's step); Q4_0, and all types for fp32 x, subtract it
+// from the code instead, exactly, for one more operation a pair.
 #pragma once
 
+#include <mutex>
+
 #include "dense.cuh"
+#include "umma.cuh"
 
 namespace artlite {
 namespace sb {
 
-constexpr int kWarps = 8, kThreads = 32 * kWarps;
+constexpr int kWarps = 16, kThreads = 32 * kWarps;
+constexpr int kMaxCluster = 8;
+constexpr int kSmemMax = 227 * 1024;
+constexpr int kCol = 20;  // floats a column of 16 partial sums takes (the fragments' stores fall in distinct banks)
 
 struct Args {
-  const void* w0;  // packed tiles (4-bit), or rows of K values (16-bit)
-  const void* w1;  // gated: the up matrix
+  CUtensorMap map[2];  // 16-bit weights: the matrices, boxes of 64 x 16
+  const uint8_t* w[2]; // 4-bit weights: packed tiles (gated: gate, up)
   const void* x;
   void* y;
   int64_t ldx, ldy;
   int64_t T;
   int K, N;
   int act;
-  float scale0, scale1;  // 4-bit: powers of two that undo the packed scales' (first matrix, up matrix)
-  float* keep_g;  // gated, 16-bit weights: the fp32 gate and up values (T x N), or null
+  float* keep_g;       // gated, 16-bit weights: the fp32 gate and up values (T x N), or null
   float* keep_u;
+  DevStatus* status;
+  int vec;             // x's rows take 16-byte loads
+  int group;           // tokens a CTA (at most 8 NT)
+  // the plan
+  int items;           // items a tile (over the whole of K)
+  int tiles;           // tiles (gated: twice the feature tiles, gate and up in turn)
+  int wk, depth, batch;  // warps a tile, ring depth, tiles a batch
+  int x_off, sum_off, scratch_off, table_off, red_off, bar_off;
 };
 
 template <class XT>
@@ -45,75 +60,39 @@ template <>
 struct MmaOf<float> {
   using type = __nv_bfloat16;
 };
-
-template <class B>
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (sizeof(B) == 2 && __is_same(B, __half))
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// ---------------------------------------------------------------- x
-
 template <class XT>
 constexpr int planes() { return sizeof(XT) == 4 ? 3 : 1; }
 
-// values k0 .. k0 + 7 and k0 + 32 .. k0 + 39 of a row (zero at and past K, or for a missing row: row == null) as eight
-// MMA pairs a plane
-template <class XT, bool VEC>
-__device__ __forceinline__ void load_x(const XT* row, int k0, int K, uint32_t (&r)[planes<XT>()][8]) {
-  if constexpr (sizeof(XT) == 2) {
-    if constexpr (VEC) {
-#pragma unroll
-      for (int j = 0; j < 2; j++) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row && k0 + 32 * j < K) v = __ldg(reinterpret_cast<const uint4*>(row + k0 + 32 * j));
-        r[0][4 * j] = v.x, r[0][4 * j + 1] = v.y, r[0][4 * j + 2] = v.z, r[0][4 * j + 3] = v.w;
-      }
-    } else {
-      const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const int k = k0 + 32 * (i >> 2) + 2 * (i & 3);
-        uint32_t lo = 0, hi = 0;
-        if (row && k < K) lo = p[k];
-        if (row && k + 1 < K) hi = p[k + 1];
-        r[0][i] = lo | hi << 16;
-      }
-    }
-  } else {
-    float v[16];
-#pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const int k = k0 + 32 * (i >> 3) + (i & 7);
-      if constexpr (VEC) {
-        float4 f = make_float4(0, 0, 0, 0);
-        if (row && k < K) f = __ldg(reinterpret_cast<const float4*>(row + k));
-        v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[i + e] = row && k + e < K ? row[k + e] : 0.0f;
-      }
-    }
-    // v = hi + mid + lo, each the upper 16 bits of what is left: 8 significant bits a plane, all 24 kept
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      uint32_t a = __float_as_uint(v[2 * j]), b = __float_as_uint(v[2 * j + 1]);
-#pragma unroll
-      for (int pl = 0; pl < 3; pl++) {
-        r[pl][j] = __byte_perm(a, b, 0x7632);
-        if (pl < 2) {
-          a = __float_as_uint(__uint_as_float(a) - __uint_as_float(a & 0xFFFF0000u));
-          b = __float_as_uint(__uint_as_float(b) - __uint_as_float(b & 0xFFFF0000u));
-        }
-      }
-    }
-  }
+#define AL_SB_MMA(T16, ...)                                                                                    \
+  asm("mma.sync.aligned.m16n8k16.row.col.f32." T16 "." T16 ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, " \
+               __VA_ARGS__)
+// c += a b
+template <class B>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (__is_same(B, __half))
+    AL_SB_MMA("f16", "{%0,%1,%2,%3};" : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+              : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    AL_SB_MMA("bf16", "{%0,%1,%2,%3};" : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+              : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// c = a b
+template <class B>
+__device__ __forceinline__ void mma0(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (__is_same(B, __half))
+    AL_SB_MMA("f16", "{%10,%10,%10,%10};" : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+              : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+  else
+    AL_SB_MMA("bf16", "{%10,%10,%10,%10};" : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+              : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+#undef AL_SB_MMA
+
+__device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   tc::smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
+               : "memory");
 }
 
 // ---------------------------------------------------------------- the code table of IQ4_NL (dequant.cpp:119)
@@ -125,300 +104,805 @@ __device__ __forceinline__ uint32_t iq4_pair(int byte) {
 }
 
 // ---------------------------------------------------------------- weight sources
-//
-// A source has: kChunkK (values a chunk), kGroups (whether sums are scaled by 32-value groups), Frag (a lane's registers
-// of one tile's chunk), load(...), and mul(...) which multiplies the chunk into the accumulators.
 
+// x fragments of a unit (64 values): plane pl, half j, column n-tile n: eight values
+struct XAt {
+  const uint8_t* x;   // this lane's first fragment: column and position t included
+  const float* sums;  // the group sums of columns 2 t, 2 t + 1
+  int cols;           // columns held
+  int col[4];         // byte offset of n-tile n's column of this lane
+};
+
+// packed 4-bit tiles (dense.cuh)
+template <int QT>
+struct QuantInt;
 template <int QT>
 struct Quant {
-  static constexpr int kChunkK = kTileK;
+  using Int = QuantInt<QT>;
+  static constexpr bool kPlain = false, kInt = false;
+  static constexpr int kItemK = kTileK, kItemBytes = tile_bytes(QT);
   static constexpr bool kTable = QT == ARTLITE_IQ4_NL;
   static constexpr bool kMin = QT == ARTLITE_Q4_1 || QT == ARTLITE_Q4_K;
-  static constexpr int kRegs = QT == ARTLITE_Q4_1 ? 4 : 2;
-  struct Frag {
-    uint4 q[kUnits];
-    uint32_t s[kRegs];
-  };
-  // tile `mt`'s chunk ch
-  static __device__ __forceinline__ void load(const Args&, const void* w, int mt, int ch, int chunks, int lane, Frag& f) {
-    const uint8_t* b = static_cast<const uint8_t*>(w) + ((int64_t)mt * chunks + ch) * tile_bytes(QT);
-    const uint4* q = reinterpret_cast<const uint4*>(b) + lane;
-#pragma unroll
-    for (int u = 0; u < kUnits; u++) f.q[u] = __ldcs(q + 32 * u);
-    if constexpr (kRegs == 4) {
-      const uint4 v = __ldcs(reinterpret_cast<const uint4*>(b + kCodeBytes) + lane);
-      f.s[0] = v.x, f.s[1] = v.y, f.s[2] = v.z, f.s[3] = v.w;
-    } else {
-      const uint2 v = __ldcs(reinterpret_cast<const uint2*>(b + kCodeBytes) + lane);
-      f.s[0] = v.x, f.s[1] = v.y;
-    }
+  static constexpr int kScratch = QT == ARTLITE_Q4_K ? 1024 : 0;  // bytes a warp
+
+  static __device__ __forceinline__ void request(const Args& a, int mat, int tile, int item, uint8_t* dst, uint64_t* bar) {
+    tc::mbar_expect_tx(bar, kItemBytes);
+    bulk_copy(dst, a.w[mat] + ((int64_t)tile * a.items + item) * kItemBytes, kItemBytes, bar);
   }
 
-  // a lane's own unit's scales (sc[row][group]) and minima, as fp32; undo: the power of two that undoes the packing's
-  static __device__ __forceinline__ void own_scales(const Frag& f, int t, float undo, float (&sc)[4], float (&mn)[4]) {
-    if constexpr (QT == ARTLITE_Q4_K) {
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        uint32_t dd = (f.s[r] >> 24) << (8 * t);  // (d | dmin << 16 from its four lanes' bytes)
-        dd |= __shfl_xor_sync(0xFFFFFFFFu, dd, 1);
-        dd |= __shfl_xor_sync(0xFFFFFFFFu, dd, 2);
-        const float2 d = Num<__half>::unpack(dd);
-        const float du = d.x * undo, dm = -d.y * undo;
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-          sc[2 * r + j] = du * (float)((f.s[r] >> (12 * j)) & 63u);
-          mn[2 * r + j] = dm * (float)((f.s[r] >> (12 * j + 6)) & 63u);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        const float2 d = Num<__half>::unpack(f.s[r]);
-        sc[2 * r] = d.x * undo, sc[2 * r + 1] = d.y * undo;
-        if constexpr (kMin) {
-          const float2 m = Num<__half>::unpack(f.s[2 + r]);
-          mn[2 * r] = m.x * undo, mn[2 * r + 1] = m.y * undo;
-        }
-      }
-    }
-  }
-
-  // word w's four A registers: the codes as integers (Q4_0: less 8), or the table's values
-  template <class B>
+  // word w's four A registers
+  template <class B, bool SUB>
   static __device__ __forceinline__ void unpack(uint32_t w, const uint32_t* table, uint32_t (&a)[4]) {
     if constexpr (kTable) {
 #pragma unroll
       for (int i = 0; i < 4; i++) a[i] = table[((w >> (8 * i)) & 0xFFu) * 32];
     } else {
       constexpr bool kHalf = __is_same(B, __half);
-      constexpr uint32_t kBase = kHalf ? 0x64006400u : 0x43004300u;  // 1024 or 128
-      constexpr int kOff = QT == ARTLITE_Q4_0 ? 8 : 0;
-      const uint32_t off = kHalf ? 0x64006400u + 0x00010001u * kOff : 0x43004300u + 0x00010001u * kOff;
+      constexpr uint32_t kBase = kHalf ? 0x4C004C00u : 0x41804180u;  // 16
+      constexpr int kAt = kHalf ? 6 : 3;                             // where 16 + q keeps q
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const uint32_t v = ((w >> (4 * i)) & 0x000F000Fu) | kBase;
-        if constexpr (kHalf) {
-          const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&off));
-          a[i] = *reinterpret_cast<const uint32_t*>(&d);
+        constexpr uint32_t kMask = 0x000F000Fu << kAt;
+        const uint32_t v = ((4 * i < kAt ? w << (kAt - 4 * i) : w >> (4 * i - kAt)) & kMask) | kBase;
+        if constexpr (SUB) {
+          constexpr int kOff = QT == ARTLITE_Q4_0 ? 8 : 0;  // 16 or 24
+          constexpr uint32_t kSub = kBase + ((uint32_t)kOff << kAt) * 0x00010001u;
+          if constexpr (kHalf) {
+            const uint32_t s = kSub;
+            const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&s));
+            a[i] = *reinterpret_cast<const uint32_t*>(&d);
+          } else {
+            const uint32_t s = kSub;
+            const __nv_bfloat162 d =
+                __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&s));
+            a[i] = *reinterpret_cast<const uint32_t*>(&d);
+          }
         } else {
-          const __nv_bfloat162 d =
-              __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&off));
-          a[i] = *reinterpret_cast<const uint32_t*>(&d);
+          a[i] = v;
+        }
+      }
+    }
+  }
+
+  template <int NT>
+  struct Acc {
+    float v[NT][4];  // rows g (0, 1) and g + 8 (2, 3), columns 8 n + 2 t and + 1
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[n][i] = 0.0f;
+    }
+    // the tile's partial sums, column-major
+    __device__ __forceinline__ void flush(float* p, int cols, const float*, int g, int t) const {
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int col = 8 * n + 2 * t + (i & 1);
+          if (col < cols) p[col * kCol + g + 8 * (i >> 1)] = v[n][i];
+        }
+    }
+  };
+
+  // the item at `buf` into the accumulators; unit0: its first unit's place in x
+  template <class XT, int NT>
+  static __device__ __forceinline__ void mul(const uint8_t* buf, const XAt& x, int unit0, uint8_t* scratch,
+                                             const uint32_t* table, int lane, Acc<NT>& acc) {
+    using B = typename MmaOf<XT>::type;
+    constexpr int P = planes<XT>();
+    constexpr bool kSub = QT == ARTLITE_Q4_0 || sizeof(XT) == 4;
+    constexpr float kBias = kSub ? 0.0f : 16.0f;
+    const int g = lane >> 2, t = lane & 3;
+    const uint8_t* tail = buf + kCodeBytes;
+    if constexpr (QT == ARTLITE_Q4_K) {
+      // lane t makes the scales and minima of group t / 2 of two units, rows g and g + 8, for the rows' lanes to find
+      const uint4 v = reinterpret_cast<const uint4*>(tail)[2 * g + (t >> 1)];
+      const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, v.w, 2);
+      const float2 d0 = Num<__half>::unpack(t < 2 ? v.w : other), d1 = Num<__half>::unpack(t < 2 ? other : v.w);
+      const float e0 = -8388608.0f * d0.x, e1 = -8388608.0f * d1.x, m0 = -8388608.0f * d0.y, m1 = -8388608.0f * d1.y;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const uint32_t w = t & 1 ? k_fields(v, 2 + h) : k_fields(v, h);
+        float4 o;
+        o.x = fmaf(k_field(w, 0), d0.x, e0);
+        o.z = fmaf(k_field(w, 12), d1.x, e1);
+        o.y = -fmaf(kBias, o.x, fmaf(k_field(w, 6), d0.y, m0));
+        o.w = -fmaf(kBias, o.z, fmaf(k_field(w, 18), d1.y, m1));
+        reinterpret_cast<float4*>(scratch)[(2 * (2 * (t & 1) + h) + (t >> 1)) * 8 + g] = o;
+      }
+      __syncwarp();
+    }
+    const uint4* codes = reinterpret_cast<const uint4*>(buf) + lane;
+#pragma unroll
+    for (int u = 0; u < kUnits; u++) {  // (units past K: zero scales and zero x)
+      const uint4 q = codes[32 * u];
+      float sc[2][2], mn[2][2];  // [row][group]
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        if constexpr (QT == ARTLITE_Q4_K) {
+          const float4 s = reinterpret_cast<const float4*>(scratch)[(2 * u + j) * 8 + g];
+          sc[0][j] = s.x, mn[0][j] = s.y, sc[1][j] = s.z, mn[1][j] = s.w;
+        } else if constexpr (QT == ARTLITE_Q4_1) {
+          const uint2 v = reinterpret_cast<const uint2*>(tail)[8 * g + 2 * u + j];
+          const float2 d = Num<__half>::unpack(v.x), m = Num<__half>::unpack(v.y);
+          sc[0][j] = d.x, sc[1][j] = d.y;
+          mn[0][j] = fmaf(-kBias, d.x, m.x), mn[1][j] = fmaf(-kBias, d.y, m.y);
+        } else {
+          const float2 d = Num<__half>::unpack(reinterpret_cast<const uint32_t*>(tail)[8 * g + 2 * u + j]);
+          sc[0][j] = d.x, sc[1][j] = d.y;
+        }
+      }
+      const uint8_t* xu = x.x + (unit0 + u) * P * 128 * x.cols;
+      const float* su = x.sums + (unit0 + u) * 16 * NT;
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        uint32_t a[2][4], A[2][4];
+        unpack<B, kSub>(j ? q.z : q.x, table, a[0]);
+        unpack<B, kSub>(j ? q.w : q.y, table, a[1]);
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) A[h][i] = a[i & 1][2 * h + (i >> 1)];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          float c[4];
+#pragma unroll
+          for (int pl = 0; pl < P; pl++) {
+            const uint4 b = *reinterpret_cast<const uint4*>(xu + (2 * pl + j) * 64 * x.cols + x.col[n]);
+            if (pl == 0) mma0<B>(c, A[0], b.x, b.y);
+            else mma<B>(c, A[0], b.x, b.y);
+            mma<B>(c, A[1], b.z, b.w);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc.v[n][i] = fmaf(sc[i >> 1][j], c[i], acc.v[n][i]);
+          if constexpr (kMin) {
+            const float2 s = *reinterpret_cast<const float2*>(su + j * 8 * NT + 8 * n);
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc.v[n][i] = fmaf(mn[i >> 1][j], i & 1 ? s.y : s.x, acc.v[n][i]);
+          }
         }
       }
     }
   }
 };
 
-// rows of K 16-bit values, ld K (K a multiple of 8, 16-byte aligned)
+// The same tiles for one to four tokens (NT of them), on the integer MMA: a token takes all eight columns.
+//
+// x becomes 32-bit fixed point over the CTA's values (2^k x, the largest in [2^29, 2^30): what is 2^-30 of a row's largest
+// and less is lost, under fp32's own rounding of such a sum) and its four signed 8-bit digits four columns; the unit's two
+// 32-value groups take two such sets of columns, each with zeros against the other group's values, so that one
+// accumulator serves both groups and each lane ends up with the sums its own scale belongs to. The packed bytes are the
+// MMA's u8 operand as they are: a byte is lo + 16 hi, and
+//   sum lo x_lo + hi x_hi = sum byte (x_hi / 16) + sum lo (x_lo - x_hi / 16),
+// the second with the byte masked to its low nibble: one logic operation for eight weights. The integer accumulator
+// starts at the bits of 1.5 2^23, so that its bits are the float 1.5 2^23 + sum (|sum| < 2^20).
+template <int QT>
+struct QuantInt : Quant<QT> {
+  static constexpr bool kInt = true;
+  static constexpr int kScratch = 0;
+
+  template <int NT>
+  struct Acc {
+    float v[NT][4];  // rows g (0, 1) and g + 8 (2, 3), the lane's two digits
+    float m[NT][2];  // the minimum's term
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[n][i] = 0.0f;
+        m[n][0] = m[n][1] = 0.0f;
+      }
+    }
+    // scale: per token two factors whose product is 2^(24 - k)
+    __device__ __forceinline__ void flush(float* p, int cols, const float* scale, int g, int t) const {
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        if (n >= cols) break;  // (uniform)
+        const float w0 = t & 1 ? 0x1p-16f : 1.0f, w1 = w0 * 0x1p-8f;
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+          float s = (v[n][2 * r] * w0 + v[n][2 * r + 1] * w1) * scale[2 * n] * scale[2 * n + 1] + m[n][r];
+          s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
+          s += __shfl_xor_sync(0xFFFFFFFFu, s, 2);
+          if (t == 0) p[n * kCol + g + 8 * r] = s;
+        }
+      }
+    }
+  };
+
+  static __device__ __forceinline__ void imma(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+
+  template <class XT, int NT>
+  static __device__ __forceinline__ void mul(const uint8_t* buf, const XAt& x, int unit0, uint8_t*, const uint32_t*,
+                                             int lane, Acc<NT>& acc) {
+    const int g = lane >> 2, t = lane & 3, j = t >> 1;  // (the lane's columns 2 t, 2 t + 1 belong to group j)
+    const uint8_t* tail = buf + kCodeBytes;
+    uint4 kv;
+    float2 d0, d1;
+    if constexpr (QT == ARTLITE_Q4_K) {
+      kv = reinterpret_cast<const uint4*>(tail)[2 * g + j];
+      const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, kv.w, 2);
+      d0 = Num<__half>::unpack(j ? other : kv.w), d1 = Num<__half>::unpack(j ? kv.w : other);
+    }
+    const uint4* codes = reinterpret_cast<const uint4*>(buf) + lane;
+    const uint32_t lo = g < 4 ? ~0u : 0u;  // B: columns 0 - 3 are group 0 (k < 16), columns 4 - 7 group 1
+#pragma unroll
+    for (int u = 0; u < kUnits; u++) {
+      const uint4 q = codes[32 * u];
+      float s0, s1, m0, m1;  // rows g and g + 8: scale, and the factor of the group's sum of x
+      if constexpr (QT == ARTLITE_Q4_K) {
+        const uint32_t w = k_fields(kv, u);
+        s0 = fmaf(k_field(w, 0), d0.x, -8388608.0f * d0.x), s1 = fmaf(k_field(w, 12), d1.x, -8388608.0f * d1.x);
+        m0 = -fmaf(k_field(w, 6), d0.y, -8388608.0f * d0.y), m1 = -fmaf(k_field(w, 18), d1.y, -8388608.0f * d1.y);
+      } else if constexpr (QT == ARTLITE_Q4_1) {
+        const uint2 v = reinterpret_cast<const uint2*>(tail)[8 * g + 2 * u + j];
+        const float2 d = Num<__half>::unpack(v.x), m = Num<__half>::unpack(v.y);
+        s0 = d.x, s1 = d.y, m0 = m.x, m1 = m.y;
+      } else {
+        const float2 d = Num<__half>::unpack(reinterpret_cast<const uint32_t*>(tail)[8 * g + 2 * u + j]);
+        s0 = d.x, s1 = d.y, m0 = -8.0f * s0, m1 = -8.0f * s1;
+      }
+      const uint32_t A[4] = {q.x, q.y, q.z, q.w};
+      const uint32_t L[4] = {q.x & 0x0F0F0F0Fu, q.y & 0x0F0F0F0Fu, q.z & 0x0F0F0F0Fu, q.w & 0x0F0F0F0Fu};
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        const uint2 b = *reinterpret_cast<const uint2*>(x.x + ((unit0 + u) * NT + n) * 256);
+        int c[4] = {0x4B400000, 0x4B400000, 0x4B400000, 0x4B400000};
+        imma(c, A, b.x & lo, b.x & ~lo);
+        imma(c, L, b.y & lo, b.y & ~lo);
+        const float xs = x.sums[((unit0 + u) * NT + n) * 4];
+        acc.v[n][0] = fmaf(s0, __int_as_float(c[0]) - 12582912.0f, acc.v[n][0]);
+        acc.v[n][1] = fmaf(s0, __int_as_float(c[1]) - 12582912.0f, acc.v[n][1]);
+        acc.v[n][2] = fmaf(s1, __int_as_float(c[2]) - 12582912.0f, acc.v[n][2]);
+        acc.v[n][3] = fmaf(s1, __int_as_float(c[3]) - 12582912.0f, acc.v[n][3]);
+        acc.m[n][0] = fmaf(m0, xs, acc.m[n][0]);
+        acc.m[n][1] = fmaf(m1, xs, acc.m[n][1]);
+      }
+    }
+  }
+};
+
+// rows of K 16-bit values (K a multiple of 8, 16-byte aligned): TMA boxes of 16 rows x 64 values, 128-byte swizzle (chunk
+// c of row r at chunk c ^ (r & 7)); lane t takes chunks 2 t and 2 t + 1 of its rows (eight lanes' loads then fall in
+// distinct banks)
 template <class WT>
 struct Plain {
-  static constexpr int kChunkK = 64;
-  static constexpr bool kTable = false;
-  struct Frag {
-    uint4 v[4];  // row g's eight values of the two 32-value groups, then row g + 8's
-  };
-  static __device__ __forceinline__ void load(const Args& a, const void* w, int mt, int ch, int, int lane, Frag& f) {
-    const int g = lane >> 2, k0 = 64 * ch + 8 * (lane & 3);
+  static constexpr bool kPlain = true, kInt = false;
+  static constexpr int kItemK = 64, kItemBytes = 2048;
+  static constexpr bool kTable = false, kMin = false;
+  static constexpr int kScratch = 0;
+
+  static __device__ __forceinline__ void request(const Args& a, int mat, int tile, int item, uint8_t* dst, uint64_t* bar) {
+    tc::mbar_expect_tx(bar, kItemBytes);
+    tc::tma_load_2d(dst, &a.map[mat], bar, 64 * item, 16 * tile);
+  }
+
+  template <int NT>
+  using Acc = typename Quant<ARTLITE_Q4_0>::template Acc<NT>;
+
+  template <class XT, int NT>
+  static __device__ __forceinline__ void mul(const uint8_t* buf, const XAt& x, int unit0, uint8_t*, const uint32_t*,
+                                             int lane, Acc<NT>& acc) {
+    const int g = lane >> 2, t = lane & 3;
+    const uint8_t* xu = x.x + unit0 * 128 * x.cols;
 #pragma unroll
-    for (int r = 0; r < 2; r++) {
-      const int64_t row = 16 * (int64_t)mt + g + 8 * r;
-      const WT* p = static_cast<const WT*>(w) + row * a.K + k0;
+    for (int j = 0; j < 2; j++) {
+      const int at = ((2 * t + j) ^ g) << 4;
+      const uint4 lo = *reinterpret_cast<const uint4*>(buf + g * 128 + at);
+      const uint4 hi = *reinterpret_cast<const uint4*>(buf + (g + 8) * 128 + at);
+      const uint32_t A[2][4] = {{lo.x, hi.x, lo.y, hi.y}, {lo.z, hi.z, lo.w, hi.w}};
 #pragma unroll
-      for (int j = 0; j < 2; j++)
-        f.v[2 * r + j] = row < a.N && k0 + 32 * j < a.K ? __ldg(reinterpret_cast<const uint4*>(p + 32 * j))
-                                                        : make_uint4(0, 0, 0, 0);
+      for (int n = 0; n < NT; n++) {
+        const uint4 b = *reinterpret_cast<const uint4*>(xu + j * 64 * x.cols + x.col[n]);
+        mma<XT>(acc.v[n], A[0], b.x, b.y);
+        mma<XT>(acc.v[n], A[1], b.z, b.w);
+      }
     }
   }
 };
 
-template <class S>
-struct IsPlain {
-  static constexpr bool value = false;
-};
-template <class WT>
-struct IsPlain<Plain<WT>> {
-  static constexpr bool value = true;
-};
+// ---------------------------------------------------------------- x into shared memory
 
-// ---------------------------------------------------------------- the kernel
-
-template <int MT, int NT>
-struct Shared {
-  float red[kWarps][MT * 16][8 * NT + 1];
-};
-template <class S, int MT, int NT>
-constexpr int smem_bytes() { return (int)sizeof(Shared<MT, NT>) + (S::kTable ? 256 * 32 * 4 : 0); }
-
-template <class S, class XT, int MT, int NT, bool GATED, bool VEC>
-__global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) small_batch(const Args a) {
-  using B = typename MmaOf<XT>::type;
-  constexpr int P = planes<XT>();
-  static_assert(!GATED || MT == 2, "a gated CTA holds one gate and one up tile");
-  extern __shared__ __align__(16) uint8_t smem[];
-  Shared<MT, NT>& sh = *reinterpret_cast<Shared<MT, NT>*>(smem);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int64_t tok0 = (int64_t)blockIdx.y * 8 * NT;
-  const int chunks = (a.K + S::kChunkK - 1) / S::kChunkK;
-  const uint32_t* table = nullptr;
-  if constexpr (S::kTable) {  // a copy of the table for every lane: reads without bank conflicts
-    uint32_t* tb = reinterpret_cast<uint32_t*>(smem + sizeof(Shared<MT, NT>));
-    for (int i = threadIdx.x; i < 256 * 32; i += kThreads) tb[i] = iq4_pair<B>(i >> 5);
-    table = tb + lane;
-    __syncthreads();
-  }
-  const XT* xr[NT];
-#pragma unroll
-  for (int n = 0; n < NT; n++) {
-    const int64_t tok = tok0 + 8 * n + g;
-    xr[n] = tok < a.T ? static_cast<const XT*>(a.x) + tok * a.ldx : nullptr;
-  }
-  float acc[MT][NT][4];
-#pragma unroll
-  for (int m = 0; m < MT; m++)
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) acc[m][n][i] = 0.0f;
-
-  typename S::Frag cur[MT], nxt[MT];
-  auto fetch = [&](int ch, typename S::Frag(&f)[MT]) {
-#pragma unroll
-    for (int m = 0; m < MT; m++)
-      S::load(a, GATED && m == 1 ? a.w1 : a.w0, GATED ? (int)blockIdx.x : (int)blockIdx.x * MT + m, ch, chunks, lane, f[m]);
-  };
-  if (warp < chunks) fetch(warp, cur);
-  for (int ch = warp; ch < chunks; ch += kWarps) {
-    if (ch + kWarps < chunks) fetch(ch + kWarps, nxt);
-    if constexpr (IsPlain<S>::value) {
-      uint32_t x[NT][P][8];
-#pragma unroll
-      for (int n = 0; n < NT; n++) load_x<XT, VEC>(xr[n], 64 * ch + 8 * t, a.K, x[n]);
-#pragma unroll
-      for (int s = 0; s < 4; s++)
-#pragma unroll
-        for (int m = 0; m < MT; m++) {
-          const uint4 lo = cur[m].v[s >> 1], hi = cur[m].v[2 + (s >> 1)];
-          const uint32_t A[4] = {s & 1 ? lo.z : lo.x, s & 1 ? hi.z : hi.x, s & 1 ? lo.w : lo.y, s & 1 ? hi.w : hi.y};
-#pragma unroll
-          for (int n = 0; n < NT; n++) mma16816<B>(acc[m][n], A, x[n][0][2 * s], x[n][0][2 * s + 1]);
-        }
+// eight values of a row from k as one 16-byte fragment a plane; returns their sum
+template <class XT>
+__device__ __forceinline__ float fragment(const XT* row, int k, bool vec, uint4 (&f)[planes<XT>()]) {
+  float s = 0.0f;
+  if constexpr (sizeof(XT) == 2) {
+    uint32_t w[4];
+    if (vec) {
+      const uint4 v = *reinterpret_cast<const uint4*>(row + k);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
     } else {
-      float sc[MT][4], mn[MT][4];
+      const uint16_t* p = reinterpret_cast<const uint16_t*>(row + k);
 #pragma unroll
-      for (int m = 0; m < MT; m++) S::own_scales(cur[m], t, GATED && m == 1 ? a.scale1 : a.scale0, sc[m], mn[m]);
+      for (int i = 0; i < 4; i++) w[i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+    }
 #pragma unroll
-      for (int u = 0; u < kUnits; u++) {
-        if (kTileK * ch + 64 * u >= a.K) break;  // (uniform)
-        uint32_t x[NT][P][8];
+    for (int i = 0; i < 4; i++) {
+      const float2 v = Num<XT>::unpack(w[i]);
+      s += v.x + v.y;
+    }
+    f[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+    float v[8];
+    if (vec) {
+      const float4 a = reinterpret_cast<const float4*>(row + k)[0], b = reinterpret_cast<const float4*>(row + k)[1];
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
 #pragma unroll
-        for (int n = 0; n < NT; n++) load_x<XT, VEC>(xr[n], kTileK * ch + 64 * u + 8 * t, a.K, x[n]);
-        const int src = (lane & ~3) | u;  // the lane that holds this unit's scales of rows g and g + 8
+      for (int i = 0; i < 8; i++) v[i] = row[k + i];
+    }
+    uint32_t w[3][4];
+    // v = hi + mid + lo, each the upper 16 bits of what is left: 8 significant bits a plane, all 24 kept
 #pragma unroll
-        for (int j = 0; j < 2; j++) {  // the unit's two 32-value groups
-          float xs[NT][4];             // (the group's sums of x, columns 2 t and 2 t + 1, in every row)
-          if constexpr (S::kMin) {
-            constexpr uint32_t kOne = __is_same(B, __half) ? 0x3C003C00u : 0x3F803F80u;
-            const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
+    for (int i = 0; i < 4; i++) {
+      uint32_t a = __float_as_uint(v[2 * i]), b = __float_as_uint(v[2 * i + 1]);
+      s += v[2 * i] + v[2 * i + 1];
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-#pragma unroll
-              for (int i = 0; i < 4; i++) xs[n][i] = 0.0f;
-#pragma unroll
-              for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int pl = 0; pl < P; pl++)
-                  mma16816<B>(xs[n], ones, x[n][pl][4 * j + 2 * h], x[n][pl][4 * j + 2 * h + 1]);
-            }
-          }
-#pragma unroll
-          for (int m = 0; m < MT; m++) {
-            const uint4 q = cur[m].q[u];
-            uint32_t A[2][4];
-            S::template unpack<B>(j ? q.z : q.x, table, A[0]);
-            S::template unpack<B>(j ? q.w : q.y, table, A[1]);
-            const float s0 = __shfl_sync(0xFFFFFFFFu, sc[m][j], src), s1 = __shfl_sync(0xFFFFFFFFu, sc[m][2 + j], src);
-            float m0 = 0.0f, m1 = 0.0f;
-            if constexpr (S::kMin)
-              m0 = __shfl_sync(0xFFFFFFFFu, mn[m][j], src), m1 = __shfl_sync(0xFFFFFFFFu, mn[m][2 + j], src);
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-              float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-              for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int pl = 0; pl < P; pl++)
-                  mma16816<B>(c, A[h], x[n][pl][4 * j + 2 * h], x[n][pl][4 * j + 2 * h + 1]);
-#pragma unroll
-              for (int i = 0; i < 4; i++) {
-                acc[m][n][i] = fmaf(i < 2 ? s0 : s1, c[i], acc[m][n][i]);
-                if constexpr (S::kMin) acc[m][n][i] = fmaf(i < 2 ? m0 : m1, xs[n][i], acc[m][n][i]);
-              }
-            }
-          }
-        }
+      for (int pl = 0; pl < 3; pl++) {
+        w[pl][i] = __byte_perm(a, b, 0x7632);
+        a = __float_as_uint(__uint_as_float(a) - __uint_as_float(a & 0xFFFF0000u));
+        b = __float_as_uint(__uint_as_float(b) - __uint_as_float(b & 0xFFFF0000u));
       }
     }
 #pragma unroll
-    for (int m = 0; m < MT; m++) cur[m] = nxt[m];
+    for (int pl = 0; pl < 3; pl++) f[pl] = make_uint4(w[pl][0], w[pl][1], w[pl][2], w[pl][3]);
   }
-  // the warps' partial sums, added in warp order
+  return s;
+}
+
+// eight values of a row from k
+template <class XT>
+__device__ __forceinline__ void values8(const XT* row, int k, bool vec, float (&v)[8]) {
+  uint4 f[planes<XT>()];
+  if constexpr (sizeof(XT) == 2) {
+    fragment<XT>(row, k, vec, f);
+    const uint32_t w[4] = {f[0].x, f[0].y, f[0].z, f[0].w};
 #pragma unroll
-  for (int m = 0; m < MT; m++)
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        sh.red[warp][16 * m + g + 8 * (i >> 1)][8 * n + 2 * t + (i & 1)] = acc[m][n][i];
-  __syncthreads();
-  constexpr int kRows = GATED ? 16 : 16 * MT;
-  for (int o = threadIdx.x; o < kRows * 8 * NT; o += kThreads) {
-    const int r = o % kRows, c = o / kRows;
-    const int64_t row = (int64_t)blockIdx.x * kRows + r, tok = tok0 + c;
-    if (row >= a.N || tok >= a.T) continue;
-    float v = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWarps; w++) v += sh.red[w][r][c];
-    if constexpr (GATED) {
-      float u = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWarps; w++) u += sh.red[w][16 + r][c];
-      if (IsPlain<S>::value && a.keep_g) {
-        a.keep_g[tok * a.N + row] = v;
-        a.keep_u[tok * a.N + row] = u;
-      }
-      v = act_of<sizeof(XT) == 4>(a.act, v) * u;
+    for (int i = 0; i < 4; i++) {
+      const float2 p = Num<XT>::unpack(w[i]);
+      v[2 * i] = p.x, v[2 * i + 1] = p.y;
     }
-    static_cast<XT*>(a.y)[tok * a.ldy + row] = Num<XT>::down(v);
+  } else if (vec) {
+    const float4 a = reinterpret_cast<const float4*>(row + k)[0], b = reinterpret_cast<const float4*>(row + k)[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = row[k + i];
   }
 }
 
-template <class S, class XT, int MT, int NT, bool GATED, bool VEC>
-int launch_one(const Args& a, cudaStream_t st) {
-  constexpr int smem = smem_bytes<S, MT, NT>();
-  auto kern = small_batch<S, XT, MT, NT, GATED, VEC>;
-  if (smem > 48 * 1024) AL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  const int rows = GATED ? 16 : 16 * MT;
+// x as digits (QuantInt): [unit][token][column 4 j + p][t] the two B registers of digit p, and [unit][token][t] the
+// group's sum at t = 0 and 2 (the lanes whose digits are the upper two), 0 at t = 1 and 3; scale: per token two factors
+// of 2^(24 - k). top: a word a token of shared memory
+template <class XT, int NT>
+__device__ void stage_digits(const Args& a, int64_t tok0, int cols, int it0, int it1, uint8_t* xs, float* sums, float* scale,
+                             uint32_t* top) {
+  const int units = (it1 - it0) * kUnits, total = units * NT * 8;
+  if (threadIdx.x < NT) top[threadIdx.x] = 0;
+  __syncthreads();
+  for (int pass = 0; pass < 2; pass++) {
+    for (int b = 0; b < total; b += kThreads) {
+      const int i = b + (int)threadIdx.x, t = i & 3, j = (i >> 2) & 1, n = (i >> 3) % NT, u = (i >> 3) / NT;
+      const int k = 64 * (it0 * kUnits + u) + 32 * j + 8 * t;
+      float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (i < total && n < cols && k < a.K) values8<XT>(static_cast<const XT*>(a.x) + (tok0 + n) * a.ldx, k, a.vec != 0, v);
+      if (pass == 0) {  // the largest magnitude: as bits, an infinity or NaN is above every number
+        uint32_t m = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) m = max(m, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+#pragma unroll
+        for (int o = 1; o < (NT == 1 ? 32 : 8); o <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+        if ((threadIdx.x & (NT == 1 ? 31 : 7)) == 0 && i < total) atomicMax(top + n, m);
+      } else {
+        const uint32_t m = top[n];
+        const bool finite = m < 0x7F800000u;
+        const int e2 = m >= 0x00800000u ? (int)(m >> 23) - 127 : -127;  // (subnormals: a little less than 2^29)
+        const int kk = m == 0 || !finite ? 0 : 29 - e2;
+        const float f0 = pow2(kk / 2), f1 = pow2(kk - kk / 2);
+        if (u == 0 && j == 0 && t == 0 && i < total) {
+          const int q = 24 - kk;
+          scale[2 * n] = finite ? pow2(q / 2) : __int_as_float(0x7FC00000);
+          scale[2 * n + 1] = pow2(q - q / 2);
+        }
+        float s = 0.0f;
+        int xi[8], hi[4];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          s += v[e];
+          xi[e] = finite ? __float2int_rn(v[e] * f0 * f1) : 0;
+        }
+        s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
+        s += __shfl_xor_sync(0xFFFFFFFFu, s, 2);
+        // byte m holds values 4 m (mod 8) + m / 2 (low nibble) and the one two further (high nibble)
+        uint32_t raw[4], low[4];
+#pragma unroll
+        for (int b4 = 0; b4 < 4; b4++) {
+          const int lo = ((4 * b4) & 7) + (b4 >> 1);
+          hi[b4] = (xi[lo + 2] + 8) >> 4;
+          raw[b4] = (uint32_t)hi[b4] + 0x80808080u;  // (digits + 128 in the bytes)
+          low[b4] = (uint32_t)(xi[lo] - hi[b4]) + 0x80808080u;
+        }
+        if (i < total) {
+#pragma unroll
+          for (int p = 0; p < 4; p++) {
+            const uint32_t sel = (uint32_t)(3 - p) | (uint32_t)(7 - p) << 4;
+            const uint32_t r = __byte_perm(__byte_perm(raw[0], raw[1], sel), __byte_perm(raw[2], raw[3], sel), 0x5410);
+            const uint32_t l = __byte_perm(__byte_perm(low[0], low[1], sel), __byte_perm(low[2], low[3], sel), 0x5410);
+            reinterpret_cast<uint2*>(xs)[(u * NT + n) * 32 + (4 * j + p) * 4 + t] =
+                make_uint2(r ^ 0x80808080u, l ^ 0x80808080u);
+          }
+          // lanes t = 2 j and 2 j + 1 belong to group j
+          if (t < 2) sums[(u * NT + n) * 4 + 2 * j + t] = t == 0 ? s : 0.0f;
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------- the kernel
+
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+
+template <class S, class XT, int NT, bool GATED>
+__global__ void __launch_bounds__(kThreads, 1) small_batch(const __grid_constant__ Args a) {
+  using B = typename MmaOf<XT>::type;
+  constexpr int P = planes<XT>();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int c = (int)cluster_size(), rank = (int)tc::cluster_rank();
+  const int cl = blockIdx.x / c, clusters = gridDim.x / c;
+  const int64_t tok0 = (int64_t)blockIdx.y * a.group;
+  const int cols = (int)min64(a.group, a.T - tok0);
+  const int partial = kCol * cols;  // floats of a tile's partial sums
+  // this cluster's tiles (gated: whole pairs) and this CTA's items
+  constexpr int kPer = GATED ? 2 : 1;
+  const int units_t = a.tiles / kPer;
+  const int tile0 = kPer * (int)((int64_t)units_t * cl / clusters), tile1 = kPer * (int)((int64_t)units_t * (cl + 1) / clusters);
+  const int it0 = (int)((int64_t)a.items * rank / c), it1 = (int)((int64_t)a.items * (rank + 1) / c);
+  const int tp = kWarps / a.wk, kl = warp % a.wk, tl = warp / a.wk;  // (tl >= tp: a warp without work)
+  uint8_t* ring = sm + warp * a.depth * S::kItemBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + a.bar_off) + warp * a.depth;
+  int* abort = reinterpret_cast<int*>(reinterpret_cast<uint64_t*>(sm + a.bar_off) + kWarps * a.depth);
+  float* red = reinterpret_cast<float*>(sm + a.red_off);
+  const bool works = tl < tp && it0 + kl < it1;
+
+  griddep_launch();
+  if (threadIdx.x == 0) *abort = 0;
+  if (lane == 0) {
+    for (int i = 0; i < a.depth; i++) tc::mbar_init(full + i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncwarp();
+  // the requests run ahead of the products by `depth` items: rt, ri the next one's tile and item
+  int rt = tile0 + tl, ri = it0 + kl;
+  auto request = [&](int stage) {
+    if (rt < tile1) {
+      S::request(a, GATED ? rt & 1 : 0, GATED ? rt >> 1 : rt, ri, ring + stage * S::kItemBytes, full + stage);
+      ri += a.wk;
+      if (ri >= it1) ri = it0 + kl, rt += tp;
+    }
+  };
+  // (a 4-bit matrix is never written after its handle was made: its first items may come before the kernels ahead of
+  // this one have ended)
+  if constexpr (S::kPlain) griddep_wait();
+  if (works && lane == 0)
+    for (int i = 0; i < a.depth; i++) request(i);
+  if constexpr (!S::kPlain) griddep_wait();
+
+  const uint32_t* table = nullptr;
+  if constexpr (S::kTable) {  // a copy of the table for every lane: reads without bank conflicts
+    uint32_t* tb = reinterpret_cast<uint32_t*>(sm + a.table_off);
+    for (int i = threadIdx.x; i < 256 * 32; i += kThreads) tb[i] = iq4_pair<B>(i >> 5);
+    table = tb + lane;
+  }
+  float* scale = reinterpret_cast<float*>(abort + 2);
+  if constexpr (S::kInt) {
+    stage_digits<XT, NT>(a, tok0, cols, it0, it1, sm + a.x_off, reinterpret_cast<float*>(sm + a.sum_off), scale,
+                         reinterpret_cast<uint32_t*>(scale + 8));
+  } else {  // x: [unit][plane][half j][column][t] 16 B, and [unit][half][column] the sums of a group's 32 values
+    constexpr int kUnitsItem = S::kItemK / 64;
+    const int units = (it1 - it0) * kUnitsItem, total = units * 2 * cols * 4;
+    float* sums = reinterpret_cast<float*>(sm + a.sum_off);
+    for (int b = 0; b < total; b += kThreads) {
+      const int i = b + (int)threadIdx.x, tt = i & 3, col = (i >> 2) % cols, uj = (i >> 2) / cols;
+      const int k = 64 * (it0 * kUnitsItem + (uj >> 1)) + (S::kPlain ? 16 * tt + 8 * (uj & 1) : 32 * (uj & 1) + 8 * tt);
+      uint4 f[P];
+#pragma unroll
+      for (int pl = 0; pl < P; pl++) f[pl] = make_uint4(0, 0, 0, 0);
+      float s = 0.0f;
+      if (i < total && k < a.K) s = fragment<XT>(static_cast<const XT*>(a.x) + (tok0 + col) * a.ldx, k, a.vec != 0, f);
+      if (i < total) {
+#pragma unroll
+        for (int pl = 0; pl < P; pl++)
+          reinterpret_cast<uint4*>(sm + a.x_off)[((((uj >> 1) * P + pl) * 2 + (uj & 1)) * cols + col) * 4 + tt] = f[pl];
+      }
+      if constexpr (S::kMin) {
+        s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
+        s += __shfl_xor_sync(0xFFFFFFFFu, s, 2);
+        if (i < total && tt == 0) sums[uj * 8 * NT + col] = s;
+      }
+    }
+  }
+  __syncthreads();
+
+  XAt x;
+  x.x = sm + a.x_off + (S::kInt ? 8 * lane : 16 * t);
+  x.sums = reinterpret_cast<const float*>(sm + a.sum_off) + (S::kInt ? t : 2 * t);
+  x.cols = cols;
+#pragma unroll
+  for (int n = 0; n < NT; n++) x.col[n] = 64 * min(8 * n + g, cols - 1);  // (columns past the last repeat it, unread)
+  uint8_t* scratch = sm + a.scratch_off + warp * S::kScratch;
+
+  int stage = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (int b0 = tile0; b0 < tile1; b0 += a.batch) {
+    const int b1 = min(b0 + a.batch, tile1);
+    if (works && ok) {
+      // (a batch holds whole rounds of tp tiles, so a warp's tiles stay the same in every batch)
+      for (int tile = b0 + tl; tile < b1 && ok; tile += tp) {
+        typename S::template Acc<NT> acc;
+        acc.zero();
+        for (int it = it0 + kl; it < it1; it += a.wk) {
+          ok = tc::wait(abort, full + stage, phase, a.status, 70);
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          if (!ok) break;
+          S::template mul<XT, NT>(ring + stage * S::kItemBytes, x, (it - it0) * (S::kItemK / 64), scratch, table, lane, acc);
+          __syncwarp();
+          if (lane == 0) request(stage);
+          if (++stage == a.depth) stage = 0, phase ^= 1;
+        }
+        acc.flush(red + ((tile - b0) * a.wk + kl) * partial, cols, scale, g, t);
+      }
+    }
+    __syncthreads();
+    // the batch's sums: this CTA's warps' in order (into the first's place), then the cluster's CTAs' in order
+    const int n_it = it1 - it0, nk = min(a.wk, n_it);
+    for (int o = threadIdx.x; o < (b1 - b0) * cols * 16; o += kThreads) {
+      const int r = o & 15, tc_ = o >> 4, col = tc_ % cols, lt = tc_ / cols;
+      float* p = red + lt * a.wk * partial + col * kCol + r;
+      float v = p[0];
+#pragma unroll 4
+      for (int k = 1; k < nk; k++) v += p[k * partial];
+      p[0] = v;
+    }
+    if (c > 1) tc::cluster_sync();
+    else __syncthreads();
+    const int rows = (b1 - b0) / kPer * 16, outs = rows * cols;
+    for (int o = threadIdx.x + kThreads * rank; o < outs; o += kThreads * c) {
+      const int r = o % rows, col = o / rows, lt = r >> 4;
+      float v[kPer];
+#pragma unroll
+      for (int m = 0; m < kPer; m++) {
+        const float* p = red + (kPer * lt + m) * a.wk * partial + col * kCol + (r & 15);
+        if (c == 1) {
+          v[m] = p[0];
+        } else {
+          float part[kMaxCluster];
+#pragma unroll
+          for (int q = 0; q < kMaxCluster; q++) {
+            uint32_t addr;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(tc::smem_u32(p)), "r"(q < c ? q : 0));
+            part[q] = q < c ? ld_cluster(addr) : 0.0f;
+          }
+          v[m] = part[0];
+#pragma unroll
+          for (int q = 1; q < kMaxCluster; q++) v[m] += part[q];
+        }
+      }
+      const int64_t row = (int64_t)(b0 / kPer) * 16 + r, tok = tok0 + col;
+      if (row < a.N) {
+        float out = v[0];
+        if constexpr (GATED) {
+          if (S::kPlain && a.keep_g) {
+            a.keep_g[tok * a.N + row] = v[0];
+            a.keep_u[tok * a.N + row] = v[kPer - 1];
+          }
+          out = act_of<sizeof(XT) == 4>(a.act, v[0]) * v[kPer - 1];
+        }
+        static_cast<XT*>(a.y)[tok * a.ldy + row] = Num<XT>::down(out);
+      }
+    }
+    if (c > 1) tc::cluster_sync();  // (the partial sums are free, and no CTA leaves while another reads its)
+    else __syncthreads();
+  }
+  // (after a wait that ran out: the copies still in flight land before the CTA's memory is given back)
+  if (*(volatile int*)abort) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 20000000LL) {
+    }
+  }
+}
+
+// ---------------------------------------------------------------- the plan
+//
+// For `clusters` clusters of c CTAs: every cluster gets tiles / clusters tiles, every CTA items / c of their items; wk
+// warps a tile and 16 / wk tiles at a time. A warp's longest run of items (rounds of tiles x items a warp) is what the
+// plan makes smallest; of equals it takes the smaller cluster (a cluster's sums cross shared memories) and the smaller wk
+// (fewer partial sums). x must fit beside a ring of two items or more.
+
+struct Plan {
+  int c = 0, clusters = 0, wk = 0, depth = 0, batch = 0, smem = 0;
+};
+
+template <class S, class XT, int NT>
+bool plan_for(Args& a, int per, int cols, const int* max_clusters, Plan* best) {
+  int64_t best_cost = -1;
+  for (int lc = 0, c = 1; c <= kMaxCluster; c *= 2, lc++) {
+    if (c > 1 && a.items < c) break;
+    if (max_clusters[lc] < 1) continue;
+    const int pairs = a.tiles / per;
+    const int clusters = pairs < max_clusters[lc] ? pairs : max_clusters[lc];
+    const int tiles = per * (int)cdiv(pairs, clusters), items = (int)cdiv(a.items, c);
+    for (int wk = 1; wk <= kWarps && wk <= items; wk++) {
+      const int tp = kWarps / wk;
+      const int64_t cost = cdiv(tiles, tp) * cdiv(items, wk);
+      const int64_t units = (int64_t)items * (S::kItemK / 64);
+      const int64_t xb = S::kInt ? units * NT * 256 : units * planes<XT>() * 128 * cols;
+      const int64_t sums = S::kInt ? units * NT * 16 : S::kMin ? units * 16 * NT * 4 : 0;
+      const int64_t fixed = 1024 + ((xb + 127) & ~127ll) + ((sums + 127) & ~127ll) + kWarps * S::kScratch +
+                            (S::kTable ? 256 * 32 * 4 : 0) + kWarps * 8 * 8 + 128;
+      // a batch: whole rounds of tp tiles, of whole pairs; as many as fit beside a ring of four, one round at least
+      int round = tp;
+      while (round % per) round += tp;
+      const int64_t tile_red = (int64_t)wk * kCol * cols * 4;
+      const int64_t ring = (int64_t)kWarps * S::kItemBytes;
+      int64_t rounds = (kSmemMax - fixed - 4 * ring) / (round * tile_red);
+      const int64_t need = cdiv(tiles, round);
+      rounds = rounds < 1 ? 1 : rounds > need ? need : rounds;
+      const int64_t red = rounds * round * tile_red;
+      const int64_t room = kSmemMax - fixed - red;
+      int depth = (int)(room / ring);
+      if (room < 2 * ring) continue;
+      if (depth > 6) depth = 6;
+      const int64_t score = cost * 16 + (depth < 3 ? cost * 4 : 0) + lc;
+      if (best_cost >= 0 && score >= best_cost) continue;
+      best_cost = score;
+      best->c = c;
+      best->clusters = clusters;
+      best->wk = wk;
+      best->depth = depth;
+      best->batch = (int)rounds * round;
+      int off = depth * kWarps * S::kItemBytes;
+      a.x_off = off;
+      off += (int)((xb + 127) & ~127ll);
+      a.sum_off = off;
+      off += (int)((sums + 127) & ~127ll);
+      a.scratch_off = off;
+      off += kWarps * S::kScratch;
+      a.table_off = off;
+      off += S::kTable ? 256 * 32 * 4 : 0;
+      a.red_off = off;
+      off += (int)red;
+      a.bar_off = off;
+      off += kWarps * depth * 8 + 128;  // (the barriers; the abort word; QuantInt's scales and largest values)
+      best->smem = off + 1024;
+    }
+  }
+  return best_cost >= 0;
+}
+
+// how many clusters of each size run at one time (asked once a kernel and device)
+template <class S, class XT, int NT, bool GATED>
+int cluster_limits(int dev, int (*out)[4]) {
+  auto kern = small_batch<S, XT, NT, GATED>;
+  constexpr int kMaxDevices = 64;
+  static int known[kMaxDevices][4];
+  static bool have[kMaxDevices];
+  static std::mutex mu;
+  AL_CHECK(dev >= 0 && dev < kMaxDevices, ARTLITE_EUNSUPPORTED, "device %d (at most %d)", dev, kMaxDevices);
+  std::lock_guard<std::mutex> lock(mu);
+  if (!have[dev]) {
+    AL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax));
+    for (int lc = 0; lc < 4; lc++) {
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(1 << lc);
+      cfg.blockDim = dim3(kThreads);
+      cfg.dynamicSmemBytes = kSmemMax;
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = 1 << lc;
+      at[0].val.clusterDim.y = 1;
+      at[0].val.clusterDim.z = 1;
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = 0;
+      }
+      known[dev][lc] = n;
+    }
+    have[dev] = true;
+  }
+  for (int lc = 0; lc < 4; lc++) (*out)[lc] = known[dev][lc];
+  return ARTLITE_OK;
+}
+
+template <class S, class XT, int NT, bool GATED>
+int launch_one(const Args& args, int dev, cudaStream_t st, bool* planned) {
+  auto kern = small_batch<S, XT, NT, GATED>;
+  int limits[4];
+  AL_TRY((cluster_limits<S, XT, NT, GATED>(dev, &limits)));
+  constexpr int per = GATED ? 2 : 1;
   // (the grid's y extent is 16 bits: longer batches go in several launches)
-  const int64_t per = (int64_t)8 * NT * 32768;
-  for (int64_t t0 = 0; t0 < a.T; t0 += per) {
-    Args b = a;
-    b.T = min64(per, a.T - t0);
-    b.x = static_cast<const XT*>(a.x) + t0 * a.ldx;
-    b.y = static_cast<XT*>(a.y) + t0 * a.ldy;
-    if (a.keep_g) b.keep_g = a.keep_g + t0 * a.N, b.keep_u = a.keep_u + t0 * a.N;
-    kern<<<dim3((unsigned)cdiv(a.N, rows), (unsigned)cdiv(b.T, 8 * NT)), kThreads, smem, st>>>(b);
-    AL_LAUNCHED();
+  const int64_t step = (int64_t)args.group * 32768;
+  for (int64_t t0 = 0; t0 < args.T; t0 += step) {
+    Args a = args;
+    a.T = min64(step, args.T - t0);
+    a.x = static_cast<const XT*>(args.x) + t0 * args.ldx;
+    a.y = static_cast<XT*>(args.y) + t0 * args.ldy;
+    if (args.keep_g) a.keep_g = args.keep_g + t0 * args.N, a.keep_u = args.keep_u + t0 * args.N;
+    a.items = (int)cdiv(a.K, S::kItemK);
+    a.tiles = per * (int)cdiv(a.N, kTileRows);
+    Plan p;
+    *planned = plan_for<S, XT, NT>(a, per, (int)min64(a.group, args.T), limits, &p);
+    if (!*planned) return ARTLITE_OK;
+    a.wk = p.wk;
+    a.depth = p.depth;
+    a.batch = p.batch;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(p.c * p.clusters), (unsigned)cdiv(a.T, a.group));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = (size_t)p.smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)p.c;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    AL_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
+    count_launch();
   }
   return ARTLITE_OK;
 }
 
-// the token tile: 8, 16 or 32 tokens a CTA
-template <class S, class XT, bool GATED, bool VEC>
-int launch(const Args& a, cudaStream_t st) {
-  if (a.T <= 8) return launch_one<S, XT, 2, 1, GATED, VEC>(a, st);
-  if (a.T <= 16) return launch_one<S, XT, 2, 2, GATED, VEC>(a, st);
-  return launch_one<S, XT, 2, 4, GATED, VEC>(a, st);
+// the token tile: 8, 16 or 32 tokens; halved until x fits
+constexpr int kMaxK = 131072;  // (one token's fp32 planes over 8 CTAs)
+template <class S, class XT, bool GATED>
+int launch(const Args& args, int dev, cudaStream_t st) {
+  Args a = args;
+  if constexpr (!S::kPlain && !S::kTable) {
+    // one to four tokens: the integer MMA. Measured at T = 1, 2, 4, 8 (us): see linear.cu
+    if (a.T <= 4) {
+      bool planned;
+      a.group = a.T <= 2 ? (int)a.T : 4;
+      AL_TRY((a.group == 1   ? launch_one<typename S::Int, XT, 1, GATED>(a, dev, st, &planned)
+              : a.group == 2 ? launch_one<typename S::Int, XT, 2, GATED>(a, dev, st, &planned)
+                             : launch_one<typename S::Int, XT, 4, GATED>(a, dev, st, &planned)));
+      if (planned) return ARTLITE_OK;
+    }
+  }
+  for (a.group = a.T <= 8 ? 8 : a.T <= 16 ? 16 : 32; a.group >= 1; a.group /= 2) {
+    bool planned;
+    AL_TRY((a.group <= 8    ? launch_one<S, XT, 1, GATED>(a, dev, st, &planned)
+            : a.group <= 16 ? launch_one<S, XT, 2, GATED>(a, dev, st, &planned)
+                            : launch_one<S, XT, 4, GATED>(a, dev, st, &planned)));
+    if (planned) return ARTLITE_OK;
+  }
+  set_error("small batch: rows of %d values", a.K);
+  return ARTLITE_EUNSUPPORTED;
 }
 
 }  // namespace sb

@@ -236,7 +236,7 @@ int artlite_moe_destroy(artlite_moe* h);
 typedef struct artlite_linear artlite_linear;
 
 typedef struct {
-  int32_t n_in;       /* values a row of x and of the matrix (a multiple of the type's block: 32, Q4_K 256) */
+  int32_t n_in;       /* values a row of x and of the matrix (a multiple of the type's block: 32, Q4_K 256; <= 131072) */
   int32_t n_out;      /* rows of the matrix, any number */
   int32_t qtype;      /* ARTLITE_Q4_0, ARTLITE_Q4_1, ARTLITE_Q4_K or ARTLITE_IQ4_NL */
   int32_t act_dtype;  /* x and y: ARTLITE_F32, ARTLITE_F16 or ARTLITE_BF16 */
