@@ -28,8 +28,19 @@ namespace sb {
 
 constexpr int kWarps = 16, kThreads = 32 * kWarps;
 constexpr int kMaxCluster = 8;
-constexpr int kSmemMax = 227 * 1024;
+// One CTA an SM: with two, a launch that starts while the one before it ends finds some SMs half free and others not, and
+// puts two of its CTAs on the former (measured: 11 us become 25). So a CTA always takes more than half of an SM's memory.
+constexpr int kSmemMax = 227 * 1024, kSmemMin = 120 * 1024;
+// Bytes a CTA keeps in flight: more of them only queue. Measured with 16-bit weights of 50 MB, T = 1: 64 KB 11.1 us, 72 KB
+// 10.9, 128 KB 12.9 - 16, 196 KB 17.0
+constexpr int kInFlight = 74 * 1024;
 constexpr int kCol = 20;  // floats a column of 16 partial sums takes (the fragments' stores fall in distinct banks)
+
+struct Plan {
+  int c, clusters;       // cluster size, clusters
+  int wk, depth, batch;  // warps a tile, ring depth, tiles a batch
+  int smem, x_off, sum_off, scratch_off, table_off, red_off, bar_off;
+};
 
 struct Args {
   CUtensorMap map[2];  // 16-bit weights: the matrices, boxes of 64 x 16
@@ -48,8 +59,7 @@ struct Args {
   // the plan
   int items;           // items a tile (over the whole of K)
   int tiles;           // tiles (gated: twice the feature tiles, gate and up in turn)
-  int wk, depth, batch;  // warps a tile, ring depth, tiles a batch
-  int x_off, sum_off, scratch_off, table_off, red_off, bar_off;
+  Plan plan;
 };
 
 template <class XT>
@@ -576,17 +586,17 @@ __global__ void __launch_bounds__(kThreads, 1) small_batch(const __grid_constant
   const int units_t = a.tiles / kPer;
   const int tile0 = kPer * (int)((int64_t)units_t * cl / clusters), tile1 = kPer * (int)((int64_t)units_t * (cl + 1) / clusters);
   const int it0 = (int)((int64_t)a.items * rank / c), it1 = (int)((int64_t)a.items * (rank + 1) / c);
-  const int tp = kWarps / a.wk, kl = warp % a.wk, tl = warp / a.wk;  // (tl >= tp: a warp without work)
-  uint8_t* ring = sm + warp * a.depth * S::kItemBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sm + a.bar_off) + warp * a.depth;
-  int* abort = reinterpret_cast<int*>(reinterpret_cast<uint64_t*>(sm + a.bar_off) + kWarps * a.depth);
-  float* red = reinterpret_cast<float*>(sm + a.red_off);
+  const int tp = kWarps / a.plan.wk, kl = warp % a.plan.wk, tl = warp / a.plan.wk;  // (tl >= tp: a warp without work)
+  uint8_t* ring = sm + warp * a.plan.depth * S::kItemBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + a.plan.bar_off) + warp * a.plan.depth;
+  int* abort = reinterpret_cast<int*>(reinterpret_cast<uint64_t*>(sm + a.plan.bar_off) + kWarps * a.plan.depth);
+  float* red = reinterpret_cast<float*>(sm + a.plan.red_off);
   const bool works = tl < tp && it0 + kl < it1;
 
   griddep_launch();
   if (threadIdx.x == 0) *abort = 0;
   if (lane == 0) {
-    for (int i = 0; i < a.depth; i++) tc::mbar_init(full + i, 1);
+    for (int i = 0; i < a.plan.depth; i++) tc::mbar_init(full + i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncwarp();
@@ -595,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1) small_batch(const __grid_constant
   auto request = [&](int stage) {
     if (rt < tile1) {
       S::request(a, GATED ? rt & 1 : 0, GATED ? rt >> 1 : rt, ri, ring + stage * S::kItemBytes, full + stage);
-      ri += a.wk;
+      ri += a.plan.wk;
       if (ri >= it1) ri = it0 + kl, rt += tp;
     }
   };
@@ -603,23 +613,23 @@ __global__ void __launch_bounds__(kThreads, 1) small_batch(const __grid_constant
   // this one have ended)
   if constexpr (S::kPlain) griddep_wait();
   if (works && lane == 0)
-    for (int i = 0; i < a.depth; i++) request(i);
+    for (int i = 0; i < a.plan.depth; i++) request(i);
   if constexpr (!S::kPlain) griddep_wait();
 
   const uint32_t* table = nullptr;
   if constexpr (S::kTable) {  // a copy of the table for every lane: reads without bank conflicts
-    uint32_t* tb = reinterpret_cast<uint32_t*>(sm + a.table_off);
+    uint32_t* tb = reinterpret_cast<uint32_t*>(sm + a.plan.table_off);
     for (int i = threadIdx.x; i < 256 * 32; i += kThreads) tb[i] = iq4_pair<B>(i >> 5);
     table = tb + lane;
   }
   float* scale = reinterpret_cast<float*>(abort + 2);
   if constexpr (S::kInt) {
-    stage_digits<XT, NT>(a, tok0, cols, it0, it1, sm + a.x_off, reinterpret_cast<float*>(sm + a.sum_off), scale,
+    stage_digits<XT, NT>(a, tok0, cols, it0, it1, sm + a.plan.x_off, reinterpret_cast<float*>(sm + a.plan.sum_off), scale,
                          reinterpret_cast<uint32_t*>(scale + 8));
   } else {  // x: [unit][plane][half j][column][t] 16 B, and [unit][half][column] the sums of a group's 32 values
     constexpr int kUnitsItem = S::kItemK / 64;
     const int units = (it1 - it0) * kUnitsItem, total = units * 2 * cols * 4;
-    float* sums = reinterpret_cast<float*>(sm + a.sum_off);
+    float* sums = reinterpret_cast<float*>(sm + a.plan.sum_off);
     for (int b = 0; b < total; b += kThreads) {
       const int i = b + (int)threadIdx.x, tt = i & 3, col = (i >> 2) % cols, uj = (i >> 2) / cols;
       const int k = 64 * (it0 * kUnitsItem + (uj >> 1)) + (S::kPlain ? 16 * tt + 8 * (uj & 1) : 32 * (uj & 1) + 8 * tt);
@@ -631,7 +641,7 @@ __global__ void __launch_bounds__(kThreads, 1) small_batch(const __grid_constant
       if (i < total) {
 #pragma unroll
         for (int pl = 0; pl < P; pl++)
-          reinterpret_cast<uint4*>(sm + a.x_off)[((((uj >> 1) * P + pl) * 2 + (uj & 1)) * cols + col) * 4 + tt] = f[pl];
+          reinterpret_cast<uint4*>(sm + a.plan.x_off)[((((uj >> 1) * P + pl) * 2 + (uj & 1)) * cols + col) * 4 + tt] = f[pl];
       }
       if constexpr (S::kMin) {
         s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
@@ -643,41 +653,41 @@ __global__ void __launch_bounds__(kThreads, 1) small_batch(const __grid_constant
   __syncthreads();
 
   XAt x;
-  x.x = sm + a.x_off + (S::kInt ? 8 * lane : 16 * t);
-  x.sums = reinterpret_cast<const float*>(sm + a.sum_off) + (S::kInt ? t : 2 * t);
+  x.x = sm + a.plan.x_off + (S::kInt ? 8 * lane : 16 * t);
+  x.sums = reinterpret_cast<const float*>(sm + a.plan.sum_off) + (S::kInt ? t : 2 * t);
   x.cols = cols;
 #pragma unroll
   for (int n = 0; n < NT; n++) x.col[n] = 64 * min(8 * n + g, cols - 1);  // (columns past the last repeat it, unread)
-  uint8_t* scratch = sm + a.scratch_off + warp * S::kScratch;
+  uint8_t* scratch = sm + a.plan.scratch_off + warp * S::kScratch;
 
   int stage = 0;
   uint32_t phase = 0;
   bool ok = true;
-  for (int b0 = tile0; b0 < tile1; b0 += a.batch) {
-    const int b1 = min(b0 + a.batch, tile1);
+  for (int b0 = tile0; b0 < tile1; b0 += a.plan.batch) {
+    const int b1 = min(b0 + a.plan.batch, tile1);
     if (works && ok) {
       // (a batch holds whole rounds of tp tiles, so a warp's tiles stay the same in every batch)
       for (int tile = b0 + tl; tile < b1 && ok; tile += tp) {
         typename S::template Acc<NT> acc;
         acc.zero();
-        for (int it = it0 + kl; it < it1; it += a.wk) {
+        for (int it = it0 + kl; it < it1; it += a.plan.wk) {
           ok = tc::wait(abort, full + stage, phase, a.status, 70);
           ok = __all_sync(0xFFFFFFFFu, ok);
           if (!ok) break;
           S::template mul<XT, NT>(ring + stage * S::kItemBytes, x, (it - it0) * (S::kItemK / 64), scratch, table, lane, acc);
           __syncwarp();
           if (lane == 0) request(stage);
-          if (++stage == a.depth) stage = 0, phase ^= 1;
+          if (++stage == a.plan.depth) stage = 0, phase ^= 1;
         }
-        acc.flush(red + ((tile - b0) * a.wk + kl) * partial, cols, scale, g, t);
+        acc.flush(red + ((tile - b0) * a.plan.wk + kl) * partial, cols, scale, g, t);
       }
     }
     __syncthreads();
     // the batch's sums: this CTA's warps' in order (into the first's place), then the cluster's CTAs' in order
-    const int n_it = it1 - it0, nk = min(a.wk, n_it);
+    const int n_it = it1 - it0, nk = min(a.plan.wk, n_it);
     for (int o = threadIdx.x; o < (b1 - b0) * cols * 16; o += kThreads) {
       const int r = o & 15, tc_ = o >> 4, col = tc_ % cols, lt = tc_ / cols;
-      float* p = red + lt * a.wk * partial + col * kCol + r;
+      float* p = red + lt * a.plan.wk * partial + col * kCol + r;
       float v = p[0];
 #pragma unroll 4
       for (int k = 1; k < nk; k++) v += p[k * partial];
@@ -691,7 +701,7 @@ __global__ void __launch_bounds__(kThreads, 1) small_batch(const __grid_constant
       float v[kPer];
 #pragma unroll
       for (int m = 0; m < kPer; m++) {
-        const float* p = red + (kPer * lt + m) * a.wk * partial + col * kCol + (r & 15);
+        const float* p = red + (kPer * lt + m) * a.plan.wk * partial + col * kCol + (r & 15);
         if (c == 1) {
           v[m] = p[0];
         } else {
@@ -736,64 +746,66 @@ __global__ void __launch_bounds__(kThreads, 1) small_batch(const __grid_constant
 // For `clusters` clusters of c CTAs: every cluster gets tiles / clusters tiles, every CTA items / c of their items; wk
 // warps a tile and 16 / wk tiles at a time. A warp's longest run of items (rounds of tiles x items a warp) is what the
 // plan makes smallest; of equals it takes the smaller cluster (a cluster's sums cross shared memories) and the smaller wk
-// (fewer partial sums). x must fit beside a ring of two items or more.
+// (fewer partial sums). x must fit beside a ring of two items or more; the ring is no deeper than kInFlight.
 
-struct Plan {
-  int c = 0, clusters = 0, wk = 0, depth = 0, batch = 0, smem = 0;
-};
+inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 template <class S, class XT, int NT>
-bool plan_for(Args& a, int per, int cols, const int* max_clusters, Plan* best) {
-  int64_t best_cost = -1;
+bool plan_for(const Args& a, int per, int cols, const int* max_clusters, Plan* best) {
+  int best_cost = -1;
   for (int lc = 0, c = 1; c <= kMaxCluster; c *= 2, lc++) {
     if (c > 1 && a.items < c) break;
     if (max_clusters[lc] < 1) continue;
     const int pairs = a.tiles / per;
     const int clusters = pairs < max_clusters[lc] ? pairs : max_clusters[lc];
-    const int tiles = per * (int)cdiv(pairs, clusters), items = (int)cdiv(a.items, c);
+    const int tiles = per * ceil_div(pairs, clusters), items = ceil_div(a.items, c);
     for (int wk = 1; wk <= kWarps && wk <= items; wk++) {
       const int tp = kWarps / wk;
-      const int64_t cost = cdiv(tiles, tp) * cdiv(items, wk);
-      const int64_t units = (int64_t)items * (S::kItemK / 64);
-      const int64_t xb = S::kInt ? units * NT * 256 : units * planes<XT>() * 128 * cols;
-      const int64_t sums = S::kInt ? units * NT * 16 : S::kMin ? units * 16 * NT * 4 : 0;
-      const int64_t fixed = 1024 + ((xb + 127) & ~127ll) + ((sums + 127) & ~127ll) + kWarps * S::kScratch +
+      const int cost = ceil_div(tiles, tp) * ceil_div(items, wk);
+      const int units = (int)items * (S::kItemK / 64);
+      const int xb = S::kInt ? units * NT * 256 : units * planes<XT>() * 128 * cols;
+      const int sums = S::kInt ? units * NT * 16 : S::kMin ? units * 16 * NT * 4 : 0;
+      const int fixed = 1024 + ((xb + 127) & ~127) + ((sums + 127) & ~127) + kWarps * S::kScratch +
                             (S::kTable ? 256 * 32 * 4 : 0) + kWarps * 8 * 8 + 128;
       // a batch: whole rounds of tp tiles, of whole pairs; as many as fit beside a ring of four, one round at least
       int round = tp;
       while (round % per) round += tp;
-      const int64_t tile_red = (int64_t)wk * kCol * cols * 4;
-      const int64_t ring = (int64_t)kWarps * S::kItemBytes;
-      int64_t rounds = (kSmemMax - fixed - 4 * ring) / (round * tile_red);
-      const int64_t need = cdiv(tiles, round);
+      const int tile_red = (int)wk * kCol * cols * 4;
+      const int ring = (int)kWarps * S::kItemBytes;
+      int rounds = (kSmemMax - fixed - 2 * ring) / (round * tile_red);
+      const int need = ceil_div(tiles, round);
       rounds = rounds < 1 ? 1 : rounds > need ? need : rounds;
-      const int64_t red = rounds * round * tile_red;
-      const int64_t room = kSmemMax - fixed - red;
-      int depth = (int)(room / ring);
+      const int red = rounds * round * tile_red;
+      const int room = kSmemMax - fixed - red;
       if (room < 2 * ring) continue;
+      const int busy = wk * (tiles < tp ? tiles : tp);  // warps with work
+      int depth = (int)(room / ring);
+      const int enough = kInFlight / (busy * S::kItemBytes);
+      if (depth > enough) depth = enough;
+      if (depth < 2) depth = 2;
       if (depth > 6) depth = 6;
-      const int64_t score = cost * 16 + (depth < 3 ? cost * 4 : 0) + lc;
+      const int score = (int)cost * 16 + lc;
       if (best_cost >= 0 && score >= best_cost) continue;
       best_cost = score;
       best->c = c;
       best->clusters = clusters;
       best->wk = wk;
       best->depth = depth;
-      best->batch = (int)rounds * round;
+      best->batch = rounds * round;
       int off = depth * kWarps * S::kItemBytes;
-      a.x_off = off;
+      best->x_off = off;
       off += (int)((xb + 127) & ~127ll);
-      a.sum_off = off;
+      best->sum_off = off;
       off += (int)((sums + 127) & ~127ll);
-      a.scratch_off = off;
+      best->scratch_off = off;
       off += kWarps * S::kScratch;
-      a.table_off = off;
+      best->table_off = off;
       off += S::kTable ? 256 * 32 * 4 : 0;
-      a.red_off = off;
+      best->red_off = off;
       off += (int)red;
-      a.bar_off = off;
+      best->bar_off = off;
       off += kWarps * depth * 8 + 128;  // (the barriers; the abort word; QuantInt's scales and largest values)
-      best->smem = off + 1024;
+      best->smem = off + 1024 > kSmemMin ? off + 1024 : kSmemMin;
     }
   }
   return best_cost >= 0;
@@ -852,12 +864,25 @@ int launch_one(const Args& args, int dev, cudaStream_t st, bool* planned) {
     if (args.keep_g) a.keep_g = args.keep_g + t0 * args.N, a.keep_u = args.keep_u + t0 * args.N;
     a.items = (int)cdiv(a.K, S::kItemK);
     a.tiles = per * (int)cdiv(a.N, kTileRows);
-    Plan p;
-    *planned = plan_for<S, XT, NT>(a, per, (int)min64(a.group, args.T), limits, &p);
-    if (!*planned) return ARTLITE_OK;
-    a.wk = p.wk;
-    a.depth = p.depth;
-    a.batch = p.batch;
+    // (a plan depends on these three sizes alone; a thread keeps its last ones)
+    struct Known {
+      int K = 0, N = 0, cols = 0, dev = 0;
+      bool ok = false;
+      Plan p;
+    };
+    static thread_local Known known[16];
+    const int cols = (int)min64(a.group, args.T);
+    Known& kn = known[((unsigned)a.K * 31u + (unsigned)a.N * 7u + (unsigned)cols) >> 3 & 15];
+    if (kn.K != a.K || kn.N != a.N || kn.cols != cols || kn.dev != dev) {
+      Known made;
+      made.K = a.K, made.N = a.N, made.cols = cols, made.dev = dev;
+      made.ok = plan_for<S, XT, NT>(a, per, cols, limits, &made.p);
+      kn = made;
+    }
+    *planned = kn.ok;
+    if (!kn.ok) return ARTLITE_OK;
+    const Plan& p = kn.p;
+    a.plan = p;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(p.c * p.clusters), (unsigned)cdiv(a.T, a.group));
     cfg.blockDim = dim3(kThreads);

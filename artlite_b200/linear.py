@@ -32,7 +32,7 @@ class QuantLinear:
                        activation=ACTIVATIONS[activation], device=device)
         h = ctypes.c_void_p()
         check(lib().artlite_linear_create(ctypes.byref(d), _ptr(keep[0]), _ptr(keep[1]), ctypes.byref(h)))
-        self._h = h
+        self._h, self._forward = h, lib().artlite_linear_forward
 
     @property
     def np_dtype(self):
@@ -52,8 +52,9 @@ class QuantLinear:
     def forward_ptr(self, x, y, T: int, *, ldx: int | None = None, ldy: int | None = None, stream: int = 0) -> None:
         """The product on device buffers (addresses, or objects with ``data_ptr()``): T rows of x ``ldx`` values apart
         (default n_in) and of y ``ldy`` apart (default n_out); enqueued on ``stream`` (0: the device's default)."""
-        check(lib().artlite_linear_forward(self._h, _ptr(x), self.n_in if ldx is None else ldx, _ptr(y),
-                                           self.n_out if ldy is None else ldy, T, ctypes.c_void_p(stream or None)))
+        rc = self._forward(self._h, _ptr(x), ldx or self.n_in, _ptr(y), ldy or self.n_out, T, stream or None)
+        if rc:
+            check(rc)
 
     def close(self) -> None:
         if getattr(self, "_h", None):
