@@ -51,6 +51,46 @@ __device__ __forceinline__ void store32(T* dst, const float (&v)[32], int valid,
     if (j < valid) dst[j] = Num<T>::down(v[j]);
 }
 
+// A warp's 32 x 32 output chunk by TMA: lane l's row l into a 4 KB shared-memory slot in the map's swizzle, then one
+// asynchronous store of the box, which the edges of the tensor clip. A lane that stored its row directly would touch 32
+// lines an instruction: with fp32 rows the epilogue then took longer than the tile's MMAs.
+constexpr int kSlot = 4096;
+template <class T>
+__device__ __forceinline__ void store_chunk(uint8_t* slot, const CUtensorMap* map, int x, int y, const float (&v)[32],
+                                            int lane) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int c = 0; c < 8; c++)
+      *reinterpret_cast<float4*>(slot + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+          make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+  } else {
+#pragma unroll
+    for (int c = 0; c < 4; c++)
+      *reinterpret_cast<uint4*>(slot + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
+          make_uint4(Num<T>::pack(v[8 * c], v[8 * c + 1]), Num<T>::pack(v[8 * c + 2], v[8 * c + 3]),
+                     Num<T>::pack(v[8 * c + 4], v[8 * c + 5]), Num<T>::pack(v[8 * c + 6], v[8 * c + 7]));
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+  if (lane == 0) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map),
+                 "r"(tc::smem_u32(slot)), "r"(x), "r"(y)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  }
+}
+// until at most N of this warp's stores still read their slots
+template <int N>
+__device__ __forceinline__ void store_wait(int lane) {
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+  __syncwarp();
+}
+// until all of this warp's stores are done
+__device__ __forceinline__ void store_finish(int lane) {
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  __syncwarp();
+}
+
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* slot) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(slot)), "r"(512));
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
@@ -59,11 +99,14 @@ __device__ __forceinline__ void tmem_free_pair(uint32_t tmem) {
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
-// a 2D map of rows x cols 16-bit values, ld apart, boxes of box_x x box_y, 128-byte swizzle, zeros outside
-// (dense_gemm's host side: linear_gemm.cu)
-int make_operand_map(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int64_t ld, int box_x, int box_y);
+// a 2D map of rows x cols values of 16 bits (32: f32), ld apart, boxes of box_x x box_y whose rows are the swizzle's span
+// (64 or 128 bytes), zeros outside (linear_gemm.cu)
+int make_tile_map(CUtensorMap* m, const void* base, bool f32, int64_t cols, int64_t rows, int64_t ld, int box_x, int box_y);
+inline int make_operand_map(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int64_t ld, int box_x, int box_y) {
+  return make_tile_map(m, base, false, cols, rows, ld, box_x, box_y);
+}
 
-// a launch of `pairs` CTA pairs
+// a programmatic launch of `pairs` CTA pairs (the kernel calls griddep_wait before it touches memory)
 template <class K, class P>
 int launch_pairs(K kern, const P& p, int pairs, int threads, size_t smem, cudaStream_t st) {
   AL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
@@ -72,13 +115,15 @@ int launch_pairs(K kern, const P& p, int pairs, int threads, size_t smem, cudaSt
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
   AL_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
   count_launch();
   return ARTLITE_OK;

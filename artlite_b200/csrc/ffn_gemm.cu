@@ -8,7 +8,8 @@
 // The transposes are the UMMA descriptors': a TMA box of 64 values x 64 k rows lands with its values consecutive, and
 // the instruction descriptor's major bits say so. Tiles past an edge read the tensor map's zeros.
 //
-// Warps (192 threads): 0 TMA, 1 the MMAs (the leader CTA's), 2 - 5 the epilogue. Six stages of 32 KB a CTA.
+// Warps (192 threads): 0 TMA, 1 the MMAs (the leader CTA's), 2 - 5 the epilogue, whose results leave by TMA stores. Six
+// stages of 32 KB a CTA (five where the forward keeps its gate and up values and stores three outputs).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -21,30 +22,36 @@ namespace {
 using namespace dg;
 
 enum { kForward = 0, kDx = 1, kDw = 2 };
-constexpr int S = 6, kThreads = 192;
+constexpr int kEpilogue = 4, kThreads = 64 + 32 * kEpilogue;
+constexpr int stages(bool keep) { return keep ? 5 : 6; }
+constexpr int NS = 4;                                                    // output slots a warp
+constexpr int slot_bytes(bool keep) { return keep ? kSlot : kSlot / 2; }  // (fp32 chunks; 16-bit ones)
 
 struct Params {
   CUtensorMap a[2], b[2];  // forward: x; Wg, Wu. dx: dg, du; Wg, Wu. dw: dg, du; x
-  void* out[2];            // forward: h. dx: dx. dw: dWg, dWu
-  int64_t ld;
-  float *g, *u;            // forward: kept values, or null
+  CUtensorMap out[2];      // forward: h. dx: dx. dw: dWg, dWu
+  CUtensorMap g, u;        // forward: the kept values
   int rows, cols;          // of the output
   int ksteps;              // stages a reduction (dx: of one of its two)
   int act;
-  bool vec;
   TileOrder order;
   DevStatus* status;
 };
 
+template <int S>
 struct Smem {
   uint64_t full[S], empty[S], tfull[2], tempty[2];
   uint32_t tmem_base;
   int abort;
 };
-constexpr size_t kSmemBytes = 1024 + 2 * (size_t)S * kStageBytes + sizeof(Smem) + 64;
+template <bool KEEP>
+constexpr size_t smem_bytes() {
+  return 1024 + 2 * (size_t)stages(KEEP) * kStageBytes + kEpilogue * NS * (size_t)slot_bytes(KEEP) + sizeof(Smem<stages(KEEP)>) + 64;
+}
 
-template <int MODE, class T>
+template <int MODE, class T, bool KEEP>
 __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ Params p) {
+  constexpr int S = stages(KEEP), SLOT = slot_bytes(KEEP);
   constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
   constexpr bool kAmn = MODE == kDw, kBmn = MODE != kForward;
   constexpr int kMats = MODE == kDw ? 2 : 1, kSegs = MODE == kDx ? 2 : 1;
@@ -52,11 +59,13 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
   uint8_t* base = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sA = base;
   uint8_t* sB = sA + S * kStageBytes;
-  Smem* sm = reinterpret_cast<Smem*>(sB + S * kStageBytes);
+  uint8_t* sOut = sB + S * kStageBytes;
+  Smem<S>* sm = reinterpret_cast<Smem<S>*>(sOut + kEpilogue * NS * SLOT);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t crank = tc::cluster_rank();
   const int per = p.order.tm * p.order.tn, total = per * kMats, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
+  griddep_launch();
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; i++) {
       tc::mbar_init(&sm->full[i], 1);
@@ -64,7 +73,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
     }
     for (int i = 0; i < 2; i++) {
       tc::mbar_init(&sm->tfull[i], 1);
-      tc::mbar_init(&sm->tempty[i], 2 * 4);
+      tc::mbar_init(&sm->tempty[i], 2 * kEpilogue);
     }
     sm->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -74,6 +83,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
   tc::cluster_sync();
   tc::fence_after();
   const uint32_t tmem = sm->tmem_base;
+  griddep_wait();
 
   if (warp == 0 && lane == 0) {
     // ---------------- TMA: this CTA's halves of A and B
@@ -85,7 +95,8 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
       const int row = m * TILE + HALF * (int)crank;
       for (int ks = 0; ks < kSegs * p.ksteps; ks++) {
         if (!tc::wait(&sm->abort, &sm->empty[s], ph ^ 1, p.status, 60)) goto out;
-        if (crank == 0) tc::mbar_expect_tx(&sm->full[s], 4 * kStageBytes);
+        if (crank == 0)
+          tc::mbar_expect_tx(&sm->full[s], 4 * kStageBytes);
         const uint32_t bar = tc::peer_addr(&sm->full[s], 0);
         const int seg = kSegs == 2 && ks >= p.ksteps ? 1 : 0, k = (ks - seg * p.ksteps) * BK;
         uint8_t *da = sA + s * kStageBytes, *db = sB + s * kStageBytes;
@@ -133,7 +144,8 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
   } else if (warp >= 2) {
     // ---------------- the epilogue: TMEM lanes 32 q .. + 31, an output row each
     const int q = warp & 3;
-    int acc = 0, aph = 0;
+    int acc = 0, aph = 0, slot = 0;
+    uint8_t* mine = sOut + (warp - 2) * NS * SLOT;
     const uint32_t tempty0 = tc::peer_addr(&sm->tempty[0], 0);
     for (int id = pair; id < total; id += pairs) {
       int m, n;
@@ -142,12 +154,11 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
       if (!tc::wait(&sm->abort, &sm->tfull[acc], aph, p.status, 63)) goto out;
       tc::fence_after();
       const uint32_t col0 = tmem + ((uint32_t)(32 * q) << 16) + acc * TILE;
-      const int r = m * TILE + HALF * (int)crank + 32 * q + lane;
-      const bool live = r < p.rows;
-      T* row = static_cast<T*>(p.out[mat]) + (int64_t)r * p.ld;
-      constexpr int kCols = MODE == kForward ? HALF : TILE;
-      for (int c = 0; c < kCols; c += 32) {
-        const int f = n * kCols + c;
+      const int row = m * TILE + HALF * (int)crank + 32 * q;
+      constexpr int cols = MODE == kForward ? HALF : TILE;
+      for (int c = 0; c < cols; c += 32) {
+        const int f = n * cols + c;
+        if (f >= p.cols || row >= p.rows) break;  // (uniform: nothing of the box is inside)
         uint32_t v[32];
         float o[32];
         tc::tmem_ld32(col0 + c, v);
@@ -156,10 +167,13 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
           tc::tmem_ld32(col0 + HALF + c, w);
           tc::tmem_wait32(v);
           tc::tmem_wait32(w);
-          if (p.g && live) {
-            const int64_t at = (int64_t)r * p.cols + f;
-            store32<float>(p.g + at, reinterpret_cast<const float(&)[32]>(v), p.cols - f, true);
-            store32<float>(p.u + at, reinterpret_cast<const float(&)[32]>(w), p.cols - f, true);
+          if constexpr (KEEP) {
+            store_wait<NS - 1>(lane);
+            store_chunk<float>(mine + slot * SLOT, &p.g, f, row, reinterpret_cast<const float(&)[32]>(v), lane);
+            slot = (slot + 1) & (NS - 1);
+            store_wait<NS - 1>(lane);
+            store_chunk<float>(mine + slot * SLOT, &p.u, f, row, reinterpret_cast<const float(&)[32]>(w), lane);
+            slot = (slot + 1) & (NS - 1);
           }
 #pragma unroll
           for (int j = 0; j < 32; j++)
@@ -169,7 +183,9 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
 #pragma unroll
           for (int j = 0; j < 32; j++) o[j] = __uint_as_float(v[j]);
         }
-        if (live) store32<T>(row + f, o, p.cols - f, p.vec);
+        store_wait<NS - 1>(lane);
+        store_chunk<T>(mine + slot * SLOT, &p.out[mat], f, row, o, lane);
+        slot = (slot + 1) & (NS - 1);
       }
       tc::fence_before();
       __syncwarp();
@@ -179,6 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
       }
       if (++acc == 2) acc = 0, aph ^= 1;
     }
+    store_finish(lane);
   }
 out:
   __syncwarp();
@@ -195,75 +212,78 @@ out:
   }
 }
 
-template <int MODE>
-int go(Params& p, int dtype, int mats, cudaStream_t st) {
+template <int MODE, bool KEEP = false>
+int go(const Params& p, int dtype, int mats, int pairs, cudaStream_t st) {
+  const int64_t total = (int64_t)p.order.tm * p.order.tn * mats;
+  AL_CHECK(total < (1ll << 31), ARTLITE_EUNSUPPORTED, "gated_ffn: %lld tiles", (long long)total);
+  const int n = total < pairs ? (int)total : pairs;
+  return dtype == ARTLITE_BF16 ? launch_pairs(ffn_gemm<MODE, __nv_bfloat16, KEEP>, p, n, kThreads, smem_bytes<KEEP>(), st)
+                               : launch_pairs(ffn_gemm<MODE, __half, KEEP>, p, n, kThreads, smem_bytes<KEEP>(), st);
+}
+
+int card_pairs(int* out) {
   int dev, sms;
   AL_CUDA(cudaGetDevice(&dev));
   AL_TRY(sm_count(dev, &sms));
-  const int64_t total = (int64_t)p.order.tm * p.order.tn * mats;
-  AL_CHECK(total < (1ll << 31), ARTLITE_EUNSUPPORTED, "gated_ffn: %lld tiles", (long long)total);
-  const int pairs = total < sms / 2 ? (int)total : sms / 2;
-  return dtype == ARTLITE_BF16 ? launch_pairs(ffn_gemm<MODE, __nv_bfloat16>, p, pairs, kThreads, kSmemBytes, st)
-                               : launch_pairs(ffn_gemm<MODE, __half>, p, pairs, kThreads, kSmemBytes, st);
+  *out = sms / 2;
+  return ARTLITE_OK;
 }
-
-bool aligned_rows(const void* p, int64_t ld) { return ((uintptr_t)p % 16) == 0 && ld % 8 == 0; }
 
 }  // namespace
 
 int launch_ffn_forward_gemm(const FfnArgs& a, cudaStream_t st) {
   Params p{};
+  int pairs;
+  AL_TRY(card_pairs(&pairs));
+  p.ksteps = (int)cdiv(a.H, BK);
   AL_TRY(make_operand_map(&p.a[0], a.x, a.H, a.T, a.ldx, BK, HALF));
-  p.a[1] = p.a[0];
   AL_TRY(make_operand_map(&p.b[0], a.wg, a.H, a.F, a.H, BK, HALF));
   AL_TRY(make_operand_map(&p.b[1], a.wu, a.H, a.F, a.H, BK, HALF));
-  p.out[0] = p.out[1] = a.h;
-  p.ld = a.ldh;
-  p.g = a.g;
-  p.u = a.u;
+  AL_TRY(make_operand_map(&p.out[0], a.h, a.F, a.T, a.ldh, 32, 32));
+  if (a.g) {
+    AL_TRY(make_tile_map(&p.g, a.g, true, a.F, a.T, a.F, 32, 32));
+    AL_TRY(make_tile_map(&p.u, a.u, true, a.F, a.T, a.F, 32, 32));
+  }
   p.rows = (int)a.T;
   p.cols = a.F;
-  p.ksteps = (int)cdiv(a.H, BK);
   p.act = a.act;
-  p.vec = aligned_rows(a.h, a.ldh);
   p.order = {(int)cdiv(a.T, TILE), (int)cdiv(a.F, HALF)};
   p.status = a.status;
-  return go<kForward>(p, a.dtype, 1, st);
+  return a.g ? go<kForward, true>(p, a.dtype, 1, pairs, st) : go<kForward>(p, a.dtype, 1, pairs, st);
 }
 
 int launch_ffn_dx_gemm(const FfnArgs& a, cudaStream_t st) {
   Params p{};
+  int pairs;
+  AL_TRY(card_pairs(&pairs));
+  p.ksteps = (int)cdiv(a.F, BK);
   AL_TRY(make_operand_map(&p.a[0], a.dg, a.F, a.T, a.F, BK, HALF));
   AL_TRY(make_operand_map(&p.a[1], a.du, a.F, a.T, a.F, BK, HALF));
   AL_TRY(make_operand_map(&p.b[0], a.wg, a.H, a.F, a.H, 64, BK));
   AL_TRY(make_operand_map(&p.b[1], a.wu, a.H, a.F, a.H, 64, BK));
-  p.out[0] = p.out[1] = a.dx;
-  p.ld = a.lddx;
+  AL_TRY(make_operand_map(&p.out[0], a.dx, a.H, a.T, a.lddx, 32, 32));
   p.rows = (int)a.T;
   p.cols = a.H;
-  p.ksteps = (int)cdiv(a.F, BK);
-  p.vec = aligned_rows(a.dx, a.lddx);
   p.order = {(int)cdiv(a.T, TILE), (int)cdiv(a.H, TILE)};
   p.status = a.status;
-  return go<kDx>(p, a.dtype, 1, st);
+  return go<kDx>(p, a.dtype, 1, pairs, st);
 }
 
 int launch_ffn_dw_gemm(const FfnArgs& a, cudaStream_t st) {
   Params p{};
+  int pairs;
+  AL_TRY(card_pairs(&pairs));
+  p.ksteps = (int)cdiv(a.T, BK);
   AL_TRY(make_operand_map(&p.a[0], a.dg, a.F, a.T, a.F, 64, BK));
   AL_TRY(make_operand_map(&p.a[1], a.du, a.F, a.T, a.F, 64, BK));
   AL_TRY(make_operand_map(&p.b[0], a.x, a.H, a.T, a.ldx, 64, BK));
-  p.b[1] = p.b[0];
-  p.out[0] = a.dwg;
-  p.out[1] = a.dwu;
-  p.ld = a.H;
+  AL_TRY(make_operand_map(&p.out[0], a.dwg, a.H, a.F, a.H, 32, 32));
+  AL_TRY(make_operand_map(&p.out[1], a.dwu, a.H, a.F, a.H, 32, 32));
   p.rows = a.F;
   p.cols = a.H;
-  p.ksteps = (int)cdiv(a.T, BK);
-  p.vec = aligned_rows(a.dwg, a.H) && aligned_rows(a.dwu, a.H);
   p.order = {(int)cdiv(a.F, TILE), (int)cdiv(a.H, TILE)};
   p.status = a.status;
-  return go<kDw>(p, a.dtype, 2, st);
+  return go<kDw>(p, a.dtype, 2, pairs, st);
 }
 
 }  // namespace artlite

@@ -210,6 +210,8 @@ __global__ void pack_kernel(int qt, const uint8_t* raw, int64_t rb, int64_t N, i
 
 // x's rows as scaled fp16 (linear.cuh): a CTA a row
 __global__ void half_rows_kernel(const uint16_t* x, int64_t ldx, int K, uint16_t* out, int32_t* row_exp) {
+  griddep_launch();
+  griddep_wait();
   const uint16_t* row = x + (int64_t)blockIdx.x * ldx;
   __shared__ float part[8];
   float m = 0.0f;
@@ -252,9 +254,7 @@ bool linear_type(int qt) {
 }  // namespace
 
 int launch_half_rows(const uint16_t* x, int64_t ldx, int64_t T, int K, uint16_t* out, int32_t* row_exp, cudaStream_t st) {
-  half_rows_kernel<<<(unsigned)T, 256, 0, st>>>(x, ldx, K, out, row_exp);
-  AL_LAUNCHED();
-  return ARTLITE_OK;
+  return launch_pdl(half_rows_kernel, dim3((unsigned)T), dim3(256), 0, st, x, ldx, K, out, row_exp);
 }
 
 }  // namespace artlite

@@ -74,52 +74,59 @@ struct Scales {
   // f0 f1: the matrix's power of two, in two factors that fp16 holds
   __device__ __forceinline__ void load(const uint8_t* tile, int g, int u, __half2 f0, __half2 f1) {
     const uint8_t* p = tile + kCodeBytes;
+    __half2 dj[2], mj[2];  // [group], of rows g and g + 8
     if constexpr (QT == ARTLITE_Q4_K) {
+      // the file's fp16 and 6-bit scales multiplied in fp16, one rounding: 2^-12 of a weight, against the output's 2^-9 in
+      // bf16. 1024 + s by one logic operation each, both rows at a time
       const uint4 v[2] = {reinterpret_cast<const uint4*>(p)[2 * g], reinterpret_cast<const uint4*>(p)[2 * g + 1]};
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        const float2 f = __half22float2(__hmul2(__hmul2(h2(v[r].w), f0), f1));
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-          // (the products of the file's fp16 and 6-bit scales round to fp16: 2^-12 of a weight, against the output's
-          // 2^-9 in bf16)
-          const uint32_t w = k_fields(v[j], u);
-          d[r][j] = __float2half2_rn(fmaf(k_field(w, 12 * r), f.x, -8388608.0f * f.x));
-          m[r][j] = __float2half2_rn(-fmaf(k_field(w, 12 * r + 6), f.y, -8388608.0f * f.y));
-        }
-      }
-    } else {
-      uint32_t w[2][2];  // [d, m][group]
-      if constexpr (QT == ARTLITE_Q4_1) {
-        const uint4 v = reinterpret_cast<const uint4*>(p)[4 * g + u];
-        w[0][0] = v.x, w[1][0] = v.y, w[0][1] = v.z, w[1][1] = v.w;
-      } else {
-        const uint2 v = reinterpret_cast<const uint2*>(p)[4 * g + u];
-        w[0][0] = v.x, w[0][1] = v.y;
-      }
+      const __half2 r0 = __hmul2(__hmul2(h2(v[0].w), f0), f1), r1 = __hmul2(__hmul2(h2(v[1].w), f0), f1);
+      const __half2 d = __lows2half2(r0, r1), dm = __hneg2(__highs2half2(r0, r1)), bias = h2(0x64006400u);
 #pragma unroll
       for (int j = 0; j < 2; j++) {
-        const __half2 a = __hmul2(__hmul2(h2(w[0][j]), f0), f1);
-        d[0][j] = __low2half2(a), d[1][j] = __high2half2(a);
-        if constexpr (QT == ARTLITE_Q4_1) {
-          const __half2 b = __hmul2(__hmul2(h2(w[1][j]), f0), f1);
-          m[0][j] = __low2half2(b), m[1][j] = __high2half2(b);
-        }
+        const uint32_t w = k_fields(v[j], u);
+        const uint32_t s = (w & 0x3Fu) | ((w << 4) & 0x003F0000u) | 0x64006400u;
+        const uint32_t n = ((w >> 6) & 0x3Fu) | ((w >> 2) & 0x003F0000u) | 0x64006400u;
+        dj[j] = __hmul2(__hsub2(h2(s), bias), d);
+        mj[j] = __hmul2(__hsub2(h2(n), bias), dm);
       }
+    } else if constexpr (QT == ARTLITE_Q4_1) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[4 * g + u];
+      dj[0] = __hmul2(__hmul2(h2(v.x), f0), f1), mj[0] = __hmul2(__hmul2(h2(v.y), f0), f1);
+      dj[1] = __hmul2(__hmul2(h2(v.z), f0), f1), mj[1] = __hmul2(__hmul2(h2(v.w), f0), f1);
+    } else {
+      const uint2 v = reinterpret_cast<const uint2*>(p)[4 * g + u];
+      dj[0] = __hmul2(__hmul2(h2(v.x), f0), f1), dj[1] = __hmul2(__hmul2(h2(v.y), f0), f1);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      d[0][j] = __low2half2(dj[j]), d[1][j] = __high2half2(dj[j]);
+      if constexpr (QT == ARTLITE_Q4_1 || QT == ARTLITE_Q4_K) m[0][j] = __low2half2(mj[j]), m[1][j] = __high2half2(mj[j]);
     }
   }
 };
 
-// word w's pair i with its group's scale: one rounding to fp16 from the exact code
+// a word's eight values times their group's scale: one rounding to fp16 from the exact codes. A nibble in a half's bits
+// 0 - 3 under 0x6400 is 1024 + q, in bits 4 - 7 it is 1024 + 16 q; the offset is taken away exactly, and for the latter
+// (1024 + 16 q) / 16 - 64 in one exact multiply-add
 template <int QT>
-__device__ __forceinline__ uint32_t decode_pair(uint32_t w, int i, __half2 d, __half2 m, const uint32_t* table) {
+__device__ __forceinline__ uint4 decode8(uint32_t w, __half2 d, __half2 m, const uint32_t* table) {
   if constexpr (QT == ARTLITE_IQ4_NL) {
-    return u32(__hmul2(h2(table[(w >> (8 * i)) & 0xFFu]), d));
+    return make_uint4(u32(__hmul2(h2(table[w & 0xFFu]), d)), u32(__hmul2(h2(table[(w >> 8) & 0xFFu]), d)),
+                      u32(__hmul2(h2(table[(w >> 16) & 0xFFu]), d)), u32(__hmul2(h2(table[w >> 24]), d)));
   } else {
-    const __half2 q = __hsub2(h2(((w >> (4 * i)) & 0x000F000Fu) | 0x64006400u),
-                              h2(QT == ARTLITE_Q4_0 ? 0x64086408u : 0x64006400u));
-    if constexpr (QT == ARTLITE_Q4_0) return u32(__hmul2(q, d));
-    else return u32(__hfma2(q, d, m));
+    constexpr bool kQ40 = QT == ARTLITE_Q4_0;
+    const __half2 lo = h2(kQ40 ? 0x64086408u : 0x64006400u), hi = h2(kQ40 ? 0xD480D480u : 0xD400D400u);  // 1024, -64 (- 8)
+    const __half2 sixteenth = h2(0x2C002C00u);
+    uint32_t o[4];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const uint32_t v = h ? w >> 8 : w;
+      const __half2 a = __hsub2(h2((v & 0x000F000Fu) | 0x64006400u), lo);
+      const __half2 b = __hfma2(h2((v & 0x00F000F0u) | 0x64006400u), sixteenth, hi);
+      o[2 * h] = u32(kQ40 ? __hmul2(a, d) : __hfma2(a, d, m));
+      o[2 * h + 1] = u32(kQ40 ? __hmul2(b, d) : __hfma2(b, d, m));
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -138,6 +145,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
   const int total = p.order.tm * p.order.tn, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int ksteps = (p.K + BK - 1) / BK, chunks = (p.K + kTileK - 1) / kTileK;
 
+  griddep_launch();
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; i++) {
       tc::mbar_init(&sm->full_a[i], 1);
@@ -165,6 +173,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
   tc::cluster_sync();
   tc::fence_after();
   const uint32_t tmem = sm->tmem_base;
+  griddep_wait();
 
   if (warp == 0 && lane == 0) {
     // ---------------- the token rows (each CTA its 128)
@@ -222,7 +231,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
   } else if (warp >= 8) {
     // ---------------- the decoding: warp 8 + i turns row tile i of every stage into fp16 rows of B (K-major, 128-byte
     // swizzle: 16-byte chunk c of row i at chunk c ^ (i & 7))
-    const int i = warp - 8, g = lane >> 2, t = lane & 3;
+    // Lanes 8 p .. 8 p + 7 take rows p and p + 4 (their 16-byte stores fall in distinct banks)
+    const int i = warp - 8, g = (lane >> 3) + (lane & 4), t = lane & 3;
     int s = 0, ph = 0, r = 0, rph = 0;
     const uint32_t full_b0 = tc::peer_addr(&sm->full_b[0], 0);
     const int we = GATED && crank ? p.w_exp1 : p.w_exp0;
@@ -233,31 +243,18 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
         const uint8_t* tile = sR + (r * 8 + i) * TB;
         const int units = min(kUnits, ksteps - kUnits * ch);
         for (int u = 0; u < units; u++) {
-          const uint4 q = reinterpret_cast<const uint4*>(tile)[32 * u + lane];
+          const uint4 q = reinterpret_cast<const uint4*>(tile)[32 * u + 4 * g + t];
           Scales<QT> sc;
           sc.load(tile, g, u, f0, f1);
-          // chunk [row][group]: eight values, word 2 j + row of the lane's codes
-          uint4 c[2][2];
-#pragma unroll
-          for (int rr = 0; rr < 2; rr++)
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-              const uint32_t a = rr ? (j ? q.w : q.y) : (j ? q.z : q.x);
-              c[rr][j] = make_uint4(decode_pair<QT>(a, 0, sc.d[rr][j], sc.m[rr][j], table),
-                                    decode_pair<QT>(a, 1, sc.d[rr][j], sc.m[rr][j], table),
-                                    decode_pair<QT>(a, 2, sc.d[rr][j], sc.m[rr][j], table),
-                                    decode_pair<QT>(a, 3, sc.d[rr][j], sc.m[rr][j], table));
-            }
+          // [row][group]: word 2 j + row of the lane's codes
+          const uint4 c[2][2] = {{decode8<QT>(q.x, sc.d[0][0], sc.m[0][0], table), decode8<QT>(q.z, sc.d[0][1], sc.m[0][1], table)},
+                                 {decode8<QT>(q.y, sc.d[1][0], sc.m[1][0], table), decode8<QT>(q.w, sc.d[1][1], sc.m[1][1], table)}};
           if (!tc::wait(&sm->abort, &sm->empty[s], ph ^ 1, p.status, 46)) goto out;
           uint8_t* row = sB + s * kStageBytes + (16 * i + g) * 128;
-          // (odd rows store their groups in the other order: eight lanes' 16-byte stores then fall in distinct banks)
 #pragma unroll
           for (int rr = 0; rr < 2; rr++)
 #pragma unroll
-            for (int jj = 0; jj < 2; jj++) {
-              const int j = jj ^ (g & 1);
-              *reinterpret_cast<uint4*>(row + rr * 1024 + (((4 * j + t) ^ g) << 4)) = j ? c[rr][1] : c[rr][0];
-            }
+            for (int j = 0; j < 2; j++) *reinterpret_cast<uint4*>(row + rr * 1024 + (((4 * j + t) ^ g) << 4)) = c[rr][j];
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
@@ -357,7 +354,7 @@ typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, v
                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-int make_operand_map(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int64_t ld, int box_x, int box_y) {
+int make_tile_map(CUtensorMap* m, const void* base, bool f32, int64_t cols, int64_t rows, int64_t ld, int box_x, int box_y) {
   static const EncodeTiled enc = [] {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -367,14 +364,16 @@ int make_operand_map(CUtensorMap* m, const void* base, int64_t cols, int64_t row
                : nullptr;
   }();
   AL_CHECK(enc, ARTLITE_ECUDA, "dense gemm: cuTensorMapEncodeTiled is unavailable");
+  const int e = f32 ? 4 : 2;
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)(ld * 2)};
+  const cuuint64_t strides[1] = {(cuuint64_t)(ld * e)};
   const cuuint32_t box[2] = {(cuuint32_t)box_x, (cuuint32_t)box_y};
   const cuuint32_t estr[2] = {1, 1};
-  // (16-bit words either way: a copy does not look at the type, and the fill is zero bits)
-  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), dims, strides, box, estr,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  // (16-bit words for either 16-bit type: a copy does not look at it, and the fill is zero bits)
+  const CUresult r = enc(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2,
+                         const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         box_x * e == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   AL_CHECK(r == CUDA_SUCCESS, ARTLITE_ECUDA, "dense gemm: cuTensorMapEncodeTiled failed (%d): %lld x %lld, %lld apart",
            (int)r, (long long)cols, (long long)rows, (long long)ld);
   return ARTLITE_OK;
