@@ -28,26 +28,20 @@ __device__ __forceinline__ void tile_at(const TileOrder& o, int id, int* m, int*
   *m = grp * G + (rem - *n * gm);
 }
 
-// 32 consecutive values of an output row: 16-byte stores where the row allows them (vec) and all are inside
+// 16 consecutive values of an output row: 16-byte stores where the row allows them (vec) and all are inside
 template <class T>
-__device__ __forceinline__ void store32(T* dst, const float (&v)[32], int valid, bool vec) {
+__device__ __forceinline__ void store16(T* dst, const float (&v)[16], int valid, bool vec) {
   if (valid <= 0) return;
-  if (vec && valid >= 32) {
-    if constexpr (sizeof(T) == 4) {
+  if (vec && valid >= 16) {
 #pragma unroll
-      for (int c = 0; c < 8; c++)
-        reinterpret_cast<float4*>(dst)[c] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-    } else {
-#pragma unroll
-      for (int c = 0; c < 4; c++)
-        reinterpret_cast<uint4*>(dst)[c] =
-            make_uint4(Num<T>::pack(v[8 * c], v[8 * c + 1]), Num<T>::pack(v[8 * c + 2], v[8 * c + 3]),
-                       Num<T>::pack(v[8 * c + 4], v[8 * c + 5]), Num<T>::pack(v[8 * c + 6], v[8 * c + 7]));
-    }
+    for (int c = 0; c < 2; c++)
+      reinterpret_cast<uint4*>(dst)[c] =
+          make_uint4(Num<T>::pack(v[8 * c], v[8 * c + 1]), Num<T>::pack(v[8 * c + 2], v[8 * c + 3]),
+                     Num<T>::pack(v[8 * c + 4], v[8 * c + 5]), Num<T>::pack(v[8 * c + 6], v[8 * c + 7]));
     return;
   }
 #pragma unroll
-  for (int j = 0; j < 32; j++)
+  for (int j = 0; j < 16; j++)
     if (j < valid) dst[j] = Num<T>::down(v[j]);
 }
 

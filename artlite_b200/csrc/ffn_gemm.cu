@@ -23,8 +23,8 @@ using namespace dg;
 
 enum { kForward = 0, kDx = 1, kDw = 2 };
 constexpr int kEpilogue = 4, kThreads = 64 + 32 * kEpilogue;
-constexpr int stages(bool keep) { return keep ? 5 : 6; }
-constexpr int NS = 4;                                                    // output slots a warp
+constexpr int stages(bool) { return 6; }
+constexpr int NS = 2;                                                    // output slots a warp
 constexpr int slot_bytes(bool keep) { return keep ? kSlot : kSlot / 2; }  // (fp32 chunks; 16-bit ones)
 
 struct Params {

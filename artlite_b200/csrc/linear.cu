@@ -208,34 +208,44 @@ __global__ void pack_kernel(int qt, const uint8_t* raw, int64_t rb, int64_t N, i
   }
 }
 
-// x's rows as scaled fp16 (linear.cuh): a CTA a row
-__global__ void half_rows_kernel(const uint16_t* x, int64_t ldx, int K, uint16_t* out, int32_t* row_exp) {
+// x's rows as scaled fp16 (linear.cuh): a CTA a row, whose first 8192 values stay in registers between the search for the
+// largest and the scaling
+__global__ void __launch_bounds__(256) half_rows_kernel(const uint16_t* x, int64_t ldx, int K, uint16_t* out, int32_t* row_exp) {
   griddep_launch();
   griddep_wait();
   const uint16_t* row = x + (int64_t)blockIdx.x * ldx;
   __shared__ float part[8];
+  constexpr int kHeld = 4, kStep = 8 * 256;
+  uint4 held[kHeld];
   float m = 0.0f;
-  for (int k = 8 * threadIdx.x; k < K; k += 8 * blockDim.x) {
-    const uint4 v = *reinterpret_cast<const uint4*>(row + k);
+  auto largest = [&](const uint4& v) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const float2 f = Num<__nv_bfloat16>::unpack(w[i]);
       m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
     }
+  };
+  const int k0 = 8 * threadIdx.x;
+#pragma unroll
+  for (int h = 0; h < kHeld; h++) {
+    held[h] = make_uint4(0, 0, 0, 0);
+    if (k0 + h * kStep < K) held[h] = *reinterpret_cast<const uint4*>(row + k0 + h * kStep);
   }
+#pragma unroll
+  for (int h = 0; h < kHeld; h++) largest(held[h]);
+  for (int k = k0 + kHeld * kStep; k < K; k += kStep) largest(*reinterpret_cast<const uint4*>(row + k));
 #pragma unroll
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
   __syncthreads();
-  m = part[0];
-  for (int i = 1; i < (int)(blockDim.x >> 5); i++) m = fmaxf(m, part[i]);
+#pragma unroll
+  for (int i = 0; i < 8; i++) m = fmaxf(m, part[i]);
   // (a row of zeros, or with an infinity, stays as it is: fp16 has both)
   const int e = m > 0.0f && m < __int_as_float(0x7F800000) ? ilogbf(m) - 14 : 0;
   const float s0 = pow2(-e / 2), s1 = pow2(-e + e / 2);  // (2^-e may exceed fp32's range)
   if (threadIdx.x == 0) row_exp[blockIdx.x] = e;
-  for (int k = 8 * threadIdx.x; k < K; k += 8 * blockDim.x) {
-    const uint4 v = *reinterpret_cast<const uint4*>(row + k);
+  auto scaled = [&](const uint4& v, int k) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     uint32_t o[4];
 #pragma unroll
@@ -244,7 +254,11 @@ __global__ void half_rows_kernel(const uint16_t* x, int64_t ldx, int K, uint16_t
       o[i] = Num<__half>::pack(f.x * s0 * s1, f.y * s0 * s1);
     }
     *reinterpret_cast<uint4*>(out + (int64_t)blockIdx.x * K + k) = make_uint4(o[0], o[1], o[2], o[3]);
-  }
+  };
+#pragma unroll
+  for (int h = 0; h < kHeld; h++)
+    if (k0 + h * kStep < K) scaled(held[h], k0 + h * kStep);
+  for (int k = k0 + kHeld * kStep; k < K; k += kStep) scaled(*reinterpret_cast<const uint4*>(row + k), k);
 }
 
 bool linear_type(int qt) {

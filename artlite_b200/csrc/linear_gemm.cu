@@ -26,9 +26,11 @@ namespace {
 
 using namespace dg;
 
-constexpr int S = 5, R = 2;
-constexpr int kThreads = 512;
-constexpr int kDecodeWarps = 8;
+// A stage is 128 values of K (two boxes of 64): half as many hand-overs between the decoding and the MMAs as with 64.
+// Stages of A and of B, packed chunks in flight
+constexpr int KS = 2 * BK, kStage = 2 * kStageBytes;
+constexpr int SA = 3, SB = 2, R = 2;
+constexpr int kDecodeWarps = 8, kThreads = 256 + 32 * kDecodeWarps;
 
 struct Params {
   CUtensorMap map_x;
@@ -46,14 +48,14 @@ struct Params {
 };
 
 struct Smem {
-  uint64_t full_a[S], full_b[S], empty[S], raw_full[R], raw_empty[R], tfull[2], tempty[2];
+  uint64_t full_a[SA], empty_a[SA], full_b[SB], empty_b[SB], raw_full[R], raw_empty[R], tfull[2], tempty[2];
   uint32_t tmem_base;
   int abort;
 };
 
 template <int QT>
 constexpr size_t smem_bytes() {
-  return 1024 + 2 * (size_t)S * kStageBytes + (size_t)R * 8 * tile_bytes(QT) + sizeof(Smem) +
+  return 1024 + (size_t)(SA + SB) * kStage + (size_t)R * 8 * tile_bytes(QT) + sizeof(Smem) +
          (QT == ARTLITE_IQ4_NL ? 256 * 4 : 0) + 64;
 }
 
@@ -67,40 +69,40 @@ __device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t b
 __device__ __forceinline__ __half2 h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
 __device__ __forceinline__ uint32_t u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 
-// a unit's scales (and minima) of row r, group j, doubled into pairs
+// A chunk's scales of rows g and g + 8, kept in registers for its four units; of(u, j, ...): unit u's scale (and minimum)
+// of group j, both rows in a pair
 template <int QT>
 struct Scales {
-  __half2 d[2][2], m[2][2];
-  // f0 f1: the matrix's power of two, in two factors that fp16 holds
-  __device__ __forceinline__ void load(const uint8_t* tile, int g, int u, __half2 f0, __half2 f1) {
-    const uint8_t* p = tile + kCodeBytes;
-    __half2 dj[2], mj[2];  // [group], of rows g and g + 8
+  uint32_t w[QT == ARTLITE_Q4_1 ? 16 : 8];
+  __half2 f0, f1;  // the matrix's power of two, in two factors that fp16 holds
+  __device__ __forceinline__ void load(const uint8_t* tile, int g) {
+    const uint4* p = reinterpret_cast<const uint4*>(tile + kCodeBytes) + (QT == ARTLITE_Q4_1 ? 4 : 2) * g;
+#pragma unroll
+    for (int i = 0; i < (QT == ARTLITE_Q4_1 ? 4 : 2); i++) {
+      const uint4 v = p[i];
+      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+    }
+    if constexpr (QT == ARTLITE_Q4_K) {  // (words 3 and 7: d | dmin of rows g and g + 8)
+      const __half2 r0 = __hmul2(__hmul2(h2(w[3]), f0), f1), r1 = __hmul2(__hmul2(h2(w[7]), f0), f1);
+      dd = __lows2half2(r0, r1), dm = __hneg2(__highs2half2(r0, r1));
+    }
+  }
+  __half2 dd, dm;
+  __device__ __forceinline__ void of(int u, int j, __half2& d, __half2& m) const {
     if constexpr (QT == ARTLITE_Q4_K) {
       // the file's fp16 and 6-bit scales multiplied in fp16, one rounding: 2^-12 of a weight, against the output's 2^-9 in
       // bf16. 1024 + s by one logic operation each, both rows at a time
-      const uint4 v[2] = {reinterpret_cast<const uint4*>(p)[2 * g], reinterpret_cast<const uint4*>(p)[2 * g + 1]};
-      const __half2 r0 = __hmul2(__hmul2(h2(v[0].w), f0), f1), r1 = __hmul2(__hmul2(h2(v[1].w), f0), f1);
-      const __half2 d = __lows2half2(r0, r1), dm = __hneg2(__highs2half2(r0, r1)), bias = h2(0x64006400u);
-#pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const uint32_t w = k_fields(v[j], u);
-        const uint32_t s = (w & 0x3Fu) | ((w << 4) & 0x003F0000u) | 0x64006400u;
-        const uint32_t n = ((w >> 6) & 0x3Fu) | ((w >> 2) & 0x003F0000u) | 0x64006400u;
-        dj[j] = __hmul2(__hsub2(h2(s), bias), d);
-        mj[j] = __hmul2(__hsub2(h2(n), bias), dm);
-      }
+      const uint4 v = make_uint4(j ? w[4] : w[0], j ? w[5] : w[1], j ? w[6] : w[2], 0);
+      const uint32_t k = k_fields(v, u);
+      const uint32_t s = (k & 0x3Fu) | ((k << 4) & 0x003F0000u) | 0x64006400u;
+      const uint32_t n = ((k >> 6) & 0x3Fu) | ((k >> 2) & 0x003F0000u) | 0x64006400u;
+      d = __hmul2(__hsub2(h2(s), h2(0x64006400u)), dd);
+      m = __hmul2(__hsub2(h2(n), h2(0x64006400u)), dm);
     } else if constexpr (QT == ARTLITE_Q4_1) {
-      const uint4 v = reinterpret_cast<const uint4*>(p)[4 * g + u];
-      dj[0] = __hmul2(__hmul2(h2(v.x), f0), f1), mj[0] = __hmul2(__hmul2(h2(v.y), f0), f1);
-      dj[1] = __hmul2(__hmul2(h2(v.z), f0), f1), mj[1] = __hmul2(__hmul2(h2(v.w), f0), f1);
+      d = __hmul2(__hmul2(h2(j ? w[4 * u + 2] : w[4 * u]), f0), f1);
+      m = __hmul2(__hmul2(h2(j ? w[4 * u + 3] : w[4 * u + 1]), f0), f1);
     } else {
-      const uint2 v = reinterpret_cast<const uint2*>(p)[4 * g + u];
-      dj[0] = __hmul2(__hmul2(h2(v.x), f0), f1), dj[1] = __hmul2(__hmul2(h2(v.y), f0), f1);
-    }
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-      d[0][j] = __low2half2(dj[j]), d[1][j] = __high2half2(dj[j]);
-      if constexpr (QT == ARTLITE_Q4_1 || QT == ARTLITE_Q4_K) m[0][j] = __low2half2(mj[j]), m[1][j] = __high2half2(mj[j]);
+      d = __hmul2(__hmul2(h2(j ? w[2 * u + 1] : w[2 * u]), f0), f1);
     }
   }
 };
@@ -136,21 +138,24 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sA = base;
-  uint8_t* sB = sA + S * kStageBytes;
-  uint8_t* sR = sB + S * kStageBytes;
+  uint8_t* sB = sA + SA * kStage;
+  uint8_t* sR = sB + SB * kStage;
   Smem* sm = reinterpret_cast<Smem*>(sR + R * 8 * TB);
   uint32_t* table = reinterpret_cast<uint32_t*>(sm + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t crank = tc::cluster_rank();
   const int total = p.order.tm * p.order.tn, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int ksteps = (p.K + BK - 1) / BK, chunks = (p.K + kTileK - 1) / kTileK;
+  const int ksteps = (p.K + KS - 1) / KS, chunks = (p.K + kTileK - 1) / kTileK;
 
   griddep_launch();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < S; i++) {
+    for (int i = 0; i < SA; i++) {
       tc::mbar_init(&sm->full_a[i], 1);
+      tc::mbar_init(&sm->empty_a[i], 1);
+    }
+    for (int i = 0; i < SB; i++) {
       tc::mbar_init(&sm->full_b[i], 2 * kDecodeWarps);
-      tc::mbar_init(&sm->empty[i], 1);
+      tc::mbar_init(&sm->empty_b[i], 1);
     }
     for (int i = 0; i < R; i++) {
       tc::mbar_init(&sm->raw_full[i], 1);
@@ -182,16 +187,18 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
       int m, n;
       tile_at(p.order, id, &m, &n);
       for (int ks = 0; ks < ksteps; ks++) {
-        if (!tc::wait(&sm->abort, &sm->empty[s], ph ^ 1, p.status, 40)) goto out;
-        if (crank == 0) tc::mbar_expect_tx(&sm->full_a[s], 2 * kStageBytes);
-        tc::tma_load_2d_pair(sA + s * kStageBytes, &p.map_x, tc::peer_addr(&sm->full_a[s], 0), ks * BK,
-                             m * TILE + HALF * (int)crank);
-        if (++s == S) s = 0, ph ^= 1;
+        if (!tc::wait(&sm->abort, &sm->empty_a[s], ph ^ 1, p.status, 40)) goto out;
+        if (crank == 0) tc::mbar_expect_tx(&sm->full_a[s], 2 * kStage);
+        const uint32_t bar = tc::peer_addr(&sm->full_a[s], 0);
+        for (int h = 0; h < 2; h++)
+          tc::tma_load_2d_pair(sA + s * kStage + h * kStageBytes, &p.map_x, bar, ks * KS + h * BK,
+                               m * TILE + HALF * (int)crank);
+        if (++s == SA) s = 0, ph ^= 1;
       }
     }
   } else if (warp == 1 && lane == 0 && crank == 0) {
     // ---------------- the MMAs
-    int s = 0, ph = 0, acc = 0, aph = 0;
+    int s = 0, ph = 0, b = 0, bph = 0, acc = 0, aph = 0;
     const uint32_t id_mma = tc::idesc_of(false, false, false, TILE, TILE);
     for (int id = pair; id < total; id += pairs) {
       if (!tc::wait_cluster(&sm->abort, &sm->tempty[acc], aph ^ 1, p.status, 41)) goto out;
@@ -199,13 +206,18 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
       const uint32_t d = tmem + acc * TILE;
       for (int ks = 0; ks < ksteps; ks++) {
         if (!tc::wait_cluster(&sm->abort, &sm->full_a[s], ph, p.status, 42)) goto out;
-        if (!tc::wait_cluster(&sm->abort, &sm->full_b[s], ph, p.status, 43)) goto out;
+        if (!tc::wait_cluster(&sm->abort, &sm->full_b[b], bph, p.status, 43)) goto out;
         tc::fence_after();
-        const uint64_t da = tc::sdesc(tc::smem_u32(sA + s * kStageBytes)), db = tc::sdesc(tc::smem_u32(sB + s * kStageBytes));
+        const uint64_t da = tc::sdesc(tc::smem_u32(sA + s * kStage)), db = tc::sdesc(tc::smem_u32(sB + b * kStage));
 #pragma unroll
-        for (int k = 0; k < BK / 16; k++) tc::mma_pair(d, da + 2 * k, db + 2 * k, id_mma, (ks | k) != 0);
-        tc::commit_pair(&sm->empty[s]);
-        if (++s == S) s = 0, ph ^= 1;
+        for (int k = 0; k < KS / 16; k++) {
+          const uint64_t at = (k / 4) * (kStageBytes >> 4) + 2 * (k % 4);
+          tc::mma_pair(d, da + at, db + at, id_mma, (ks | k) != 0);
+        }
+        tc::commit_pair(&sm->empty_a[s]);
+        tc::commit_pair(&sm->empty_b[b]);
+        if (++s == SA) s = 0, ph ^= 1;
+        if (++b == SB) b = 0, bph ^= 1;
       }
       tc::commit_pair(&sm->tfull[acc]);
       if (++acc == 2) acc = 0, aph ^= 1;
@@ -231,37 +243,52 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
   } else if (warp >= 8) {
     // ---------------- the decoding: warp 8 + i turns row tile i of every stage into fp16 rows of B (K-major, 128-byte
     // swizzle: 16-byte chunk c of row i at chunk c ^ (i & 7))
-    // Lanes 8 p .. 8 p + 7 take rows p and p + 4 (their 16-byte stores fall in distinct banks)
-    const int i = warp - 8, g = (lane >> 3) + (lane & 4), t = lane & 3;
+    // Odd rows take their two groups in the other order: eight lanes' 16-byte stores then fall in distinct banks
+    const int i = warp - 8, g = lane >> 2, t = lane & 3, odd = g & 1;
     int s = 0, ph = 0, r = 0, rph = 0;
     const uint32_t full_b0 = tc::peer_addr(&sm->full_b[0], 0);
     const int we = GATED && crank ? p.w_exp1 : p.w_exp0;
-    const __half2 f0 = __float2half2_rn(pow2(we / 2)), f1 = __float2half2_rn(pow2(we - we / 2));
+    Scales<QT> sc;
+    sc.f0 = __float2half2_rn(pow2(we / 2)), sc.f1 = __float2half2_rn(pow2(we - we / 2));
     for (int id = pair; id < total; id += pairs) {
       for (int ch = 0; ch < chunks; ch++) {
         if (!tc::wait(&sm->abort, &sm->raw_full[r], rph, p.status, 45)) goto out;
         const uint8_t* tile = sR + (r * 8 + i) * TB;
-        const int units = min(kUnits, ksteps - kUnits * ch);
-        for (int u = 0; u < units; u++) {
-          const uint4 q = reinterpret_cast<const uint4*>(tile)[32 * u + 4 * g + t];
-          Scales<QT> sc;
-          sc.load(tile, g, u, f0, f1);
-          // [row][group]: word 2 j + row of the lane's codes
-          const uint4 c[2][2] = {{decode8<QT>(q.x, sc.d[0][0], sc.m[0][0], table), decode8<QT>(q.z, sc.d[0][1], sc.m[0][1], table)},
-                                 {decode8<QT>(q.y, sc.d[1][0], sc.m[1][0], table), decode8<QT>(q.w, sc.d[1][1], sc.m[1][1], table)}};
-          if (!tc::wait(&sm->abort, &sm->empty[s], ph ^ 1, p.status, 46)) goto out;
-          uint8_t* row = sB + s * kStageBytes + (16 * i + g) * 128;
+        const int stages = min(kUnits / 2, ksteps - kUnits / 2 * ch);
+        sc.load(tile, g);
 #pragma unroll
-          for (int rr = 0; rr < 2; rr++)
+        for (int h = 0; h < kUnits / 2; h++) {
+          if (h >= stages) break;
+          // [unit of the stage][row][group, the lane's first and second]: word 2 j + row of the lane's codes
+          uint4 c[2][2][2];
 #pragma unroll
-            for (int j = 0; j < 2; j++) *reinterpret_cast<uint4*>(row + rr * 1024 + (((4 * j + t) ^ g) << 4)) = c[rr][j];
+          for (int v = 0; v < 2; v++) {
+            const uint4 q = reinterpret_cast<const uint4*>(tile)[32 * (2 * h + v) + lane];
+            const uint32_t w[2][2] = {{odd ? q.z : q.x, odd ? q.x : q.z}, {odd ? q.w : q.y, odd ? q.y : q.w}};
+#pragma unroll
+            for (int jj = 0; jj < 2; jj++) {
+              __half2 d, m;
+              sc.of(2 * h + v, jj ^ odd, d, m);
+              c[v][0][jj] = decode8<QT>(w[0][jj], __low2half2(d), __low2half2(m), table);
+              c[v][1][jj] = decode8<QT>(w[1][jj], __high2half2(d), __high2half2(m), table);
+            }
+          }
+          if (!tc::wait(&sm->abort, &sm->empty_b[s], ph ^ 1, p.status, 46)) goto out;
+          uint8_t* row = sB + s * kStage + (16 * i + g) * 128;
+#pragma unroll
+          for (int v = 0; v < 2; v++)
+#pragma unroll
+            for (int rr = 0; rr < 2; rr++)
+#pragma unroll
+              for (int jj = 0; jj < 2; jj++)
+                *reinterpret_cast<uint4*>(row + v * kStageBytes + rr * 1024 + (((4 * (jj ^ odd) + t) ^ g) << 4)) = c[v][rr][jj];
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
             if (crank != 0) tc::arrive_cluster(full_b0 + s * (uint32_t)sizeof(uint64_t));
             else tc::mbar_arrive(&sm->full_b[s]);
           }
-          if (++s == S) s = 0, ph ^= 1;
+          if (++s == SB) s = 0, ph ^= 1;
         }
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&sm->raw_empty[r]);
@@ -288,25 +315,25 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
       const float b0 = pow2(e1 / 2), b1 = pow2(e1 - e1 / 2);
       T* row = static_cast<T*>(p.y) + (int64_t)tok * p.ldy;
       constexpr int kCols = GATED ? HALF : TILE;
-      for (int c = 0; c < kCols; c += 32) {
+      for (int c = 0; c < kCols; c += 16) {
         const int f = n * kCols + c;
-        uint32_t v[32];
-        float o[32];
-        tc::tmem_ld32(col0 + c, v);
+        uint32_t v[16];
+        float o[16];
+        tc::tmem_ld16(col0 + c, v);
         if constexpr (GATED) {
-          uint32_t w[32];
-          tc::tmem_ld32(col0 + HALF + c, w);
-          tc::tmem_wait32(v);
-          tc::tmem_wait32(w);
+          uint32_t w[16];
+          tc::tmem_ld16(col0 + HALF + c, w);
+          tc::tmem_wait16(v);
+          tc::tmem_wait16(w);
 #pragma unroll
-          for (int j = 0; j < 32; j++)
+          for (int j = 0; j < 16; j++)
             o[j] = act_of<false>(p.act, __uint_as_float(v[j]) * a0 * a1) * (__uint_as_float(w[j]) * b0 * b1);
         } else {
-          tc::tmem_wait32(v);
+          tc::tmem_wait16(v);
 #pragma unroll
-          for (int j = 0; j < 32; j++) o[j] = __uint_as_float(v[j]) * a0 * a1;
+          for (int j = 0; j < 16; j++) o[j] = __uint_as_float(v[j]) * a0 * a1;
         }
-        if (live) store32<T>(row + f, o, p.N - f, p.vec_y);
+        if (live) store16<T>(row + f, o, p.N - f, p.vec_y);
       }
       tc::fence_before();
       __syncwarp();

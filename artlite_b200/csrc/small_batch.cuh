@@ -671,8 +671,7 @@ __global__ void __launch_bounds__(kThreads, 1) small_batch(const __grid_constant
         typename S::template Acc<NT> acc;
         acc.zero();
         for (int it = it0 + kl; it < it1; it += a.plan.wk) {
-          ok = tc::wait(abort, full + stage, phase, a.status, 70);
-          ok = __all_sync(0xFFFFFFFFu, ok);
+          ok = __all_sync(0xFFFFFFFFu, tc::wait(abort, full + stage, phase, a.status, 70));
           if (!ok) break;
           S::template mul<XT, NT>(ring + stage * S::kItemBytes, x, (it - it0) * (S::kItemK / 64), scratch, table, lane, acc);
           __syncwarp();
