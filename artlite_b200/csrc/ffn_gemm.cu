@@ -8,8 +8,8 @@
 // The transposes are the UMMA descriptors': a TMA box of 64 values x 64 k rows lands with its values consecutive, and
 // the instruction descriptor's major bits say so. Tiles past an edge read the tensor map's zeros.
 //
-// Warps (192 threads): 0 TMA, 1 the MMAs (the leader CTA's), 2 - 5 the epilogue, whose results leave by TMA stores. Six
-// stages of 32 KB a CTA (five where the forward keeps its gate and up values and stores three outputs).
+// Warps (192 threads): 0 TMA, 1 the MMAs (the leader CTA's), 2 - 5 the epilogue, whose results leave by TMA stores. Three
+// stages of 64 KB a CTA.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -23,7 +23,7 @@ using namespace dg;
 
 enum { kForward = 0, kDx = 1, kDw = 2 };
 constexpr int kEpilogue = 4, kThreads = 64 + 32 * kEpilogue;
-constexpr int stages(bool) { return 6; }
+constexpr int S = 3, KS = 2 * BK, kStage = 2 * kStageBytes;  // stages, of 128 values of the reduction
 constexpr int NS = 2;                                                    // output slots a warp
 constexpr int slot_bytes(bool keep) { return keep ? kSlot : kSlot / 2; }  // (fp32 chunks; 16-bit ones)
 
@@ -38,7 +38,6 @@ struct Params {
   DevStatus* status;
 };
 
-template <int S>
 struct Smem {
   uint64_t full[S], empty[S], tfull[2], tempty[2];
   uint32_t tmem_base;
@@ -46,21 +45,21 @@ struct Smem {
 };
 template <bool KEEP>
 constexpr size_t smem_bytes() {
-  return 1024 + 2 * (size_t)stages(KEEP) * kStageBytes + kEpilogue * NS * (size_t)slot_bytes(KEEP) + sizeof(Smem<stages(KEEP)>) + 64;
+  return 1024 + 2 * (size_t)S * kStage + kEpilogue * NS * (size_t)slot_bytes(KEEP) + sizeof(Smem) + 64;
 }
 
 template <int MODE, class T, bool KEEP>
 __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ Params p) {
-  constexpr int S = stages(KEEP), SLOT = slot_bytes(KEEP);
+  constexpr int SLOT = slot_bytes(KEEP);
   constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
   constexpr bool kAmn = MODE == kDw, kBmn = MODE != kForward;
   constexpr int kMats = MODE == kDw ? 2 : 1, kSegs = MODE == kDx ? 2 : 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sA = base;
-  uint8_t* sB = sA + S * kStageBytes;
-  uint8_t* sOut = sB + S * kStageBytes;
-  Smem<S>* sm = reinterpret_cast<Smem<S>*>(sOut + kEpilogue * NS * SLOT);
+  uint8_t* sB = sA + S * kStage;
+  uint8_t* sOut = sB + S * kStage;
+  Smem* sm = reinterpret_cast<Smem*>(sOut + kEpilogue * NS * SLOT);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t crank = tc::cluster_rank();
   const int per = p.order.tm * p.order.tn, total = per * kMats, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -96,23 +95,26 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
       for (int ks = 0; ks < kSegs * p.ksteps; ks++) {
         if (!tc::wait(&sm->abort, &sm->empty[s], ph ^ 1, p.status, 60)) goto out;
         if (crank == 0)
-          tc::mbar_expect_tx(&sm->full[s], 4 * kStageBytes);
+          tc::mbar_expect_tx(&sm->full[s], 4 * kStage);
         const uint32_t bar = tc::peer_addr(&sm->full[s], 0);
-        const int seg = kSegs == 2 && ks >= p.ksteps ? 1 : 0, k = (ks - seg * p.ksteps) * BK;
-        uint8_t *da = sA + s * kStageBytes, *db = sB + s * kStageBytes;
-        if constexpr (MODE == kForward) {
-          tc::tma_load_2d_pair(da, &p.a[0], bar, k, row);
-          tc::tma_load_2d_pair(db, &p.b[crank], bar, k, n * HALF);
-        } else {
-          const int col = n * TILE + HALF * (int)crank;
-          if constexpr (MODE == kDx) {
-            tc::tma_load_2d_pair(da, &p.a[seg], bar, k, row);
+        const int seg = kSegs == 2 && ks >= p.ksteps ? 1 : 0;
+        for (int h = 0; h < 2; h++) {
+          const int k = (ks - seg * p.ksteps) * KS + h * BK;
+          uint8_t *da = sA + s * kStage + h * kStageBytes, *db = sB + s * kStage + h * kStageBytes;
+          if constexpr (MODE == kForward) {
+            tc::tma_load_2d_pair(da, &p.a[0], bar, k, row);
+            tc::tma_load_2d_pair(db, &p.b[crank], bar, k, n * HALF);
           } else {
-            tc::tma_load_2d_pair(da, &p.a[mat], bar, row, k);
-            tc::tma_load_2d_pair(da + kStageBytes / 2, &p.a[mat], bar, row + 64, k);
+            const int col = n * TILE + HALF * (int)crank;
+            if constexpr (MODE == kDx) {
+              tc::tma_load_2d_pair(da, &p.a[seg], bar, k, row);
+            } else {
+              tc::tma_load_2d_pair(da, &p.a[mat], bar, row, k);
+              tc::tma_load_2d_pair(da + kStageBytes / 2, &p.a[mat], bar, row + 64, k);
+            }
+            tc::tma_load_2d_pair(db, &p.b[seg], bar, col, k);
+            tc::tma_load_2d_pair(db + kStageBytes / 2, &p.b[seg], bar, col + 64, k);
           }
-          tc::tma_load_2d_pair(db, &p.b[seg], bar, col, k);
-          tc::tma_load_2d_pair(db + kStageBytes / 2, &p.b[seg], bar, col + 64, k);
         }
         if (++s == S) s = 0, ph ^= 1;
       }
@@ -130,11 +132,14 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
       for (int ks = 0; ks < kSegs * p.ksteps; ks++) {
         if (!tc::wait_cluster(&sm->abort, &sm->full[s], ph, p.status, 62)) goto out;
         tc::fence_after();
-        const uint32_t aa = tc::smem_u32(sA + s * kStageBytes), ab = tc::smem_u32(sB + s * kStageBytes);
+        const uint32_t aa = tc::smem_u32(sA + s * kStage), ab = tc::smem_u32(sB + s * kStage);
         const uint64_t da = kAmn ? tc::sdesc_mn(aa, kStageBytes / 2) : tc::sdesc(aa);
         const uint64_t db = kBmn ? tc::sdesc_mn(ab, kStageBytes / 2) : tc::sdesc(ab);
 #pragma unroll
-        for (int k = 0; k < BK / 16; k++) tc::mma_pair(d, da + k * kStepA, db + k * kStepB, id_mma, (ks | k) != 0);
+        for (int k = 0; k < KS / 16; k++) {
+          const uint64_t box = (k / 4) * (kStageBytes >> 4);
+          tc::mma_pair(d, da + box + (k % 4) * kStepA, db + box + (k % 4) * kStepB, id_mma, (ks | k) != 0);
+        }
         tc::commit_pair(&sm->empty[s]);
         if (++s == S) s = 0, ph ^= 1;
       }
@@ -235,7 +240,7 @@ int launch_ffn_forward_gemm(const FfnArgs& a, cudaStream_t st) {
   Params p{};
   int pairs;
   AL_TRY(card_pairs(&pairs));
-  p.ksteps = (int)cdiv(a.H, BK);
+  p.ksteps = (int)cdiv(a.H, KS);
   AL_TRY(make_operand_map(&p.a[0], a.x, a.H, a.T, a.ldx, BK, HALF));
   AL_TRY(make_operand_map(&p.b[0], a.wg, a.H, a.F, a.H, BK, HALF));
   AL_TRY(make_operand_map(&p.b[1], a.wu, a.H, a.F, a.H, BK, HALF));
@@ -256,7 +261,7 @@ int launch_ffn_dx_gemm(const FfnArgs& a, cudaStream_t st) {
   Params p{};
   int pairs;
   AL_TRY(card_pairs(&pairs));
-  p.ksteps = (int)cdiv(a.F, BK);
+  p.ksteps = (int)cdiv(a.F, KS);
   AL_TRY(make_operand_map(&p.a[0], a.dg, a.F, a.T, a.F, BK, HALF));
   AL_TRY(make_operand_map(&p.a[1], a.du, a.F, a.T, a.F, BK, HALF));
   AL_TRY(make_operand_map(&p.b[0], a.wg, a.H, a.F, a.H, 64, BK));
@@ -273,7 +278,7 @@ int launch_ffn_dw_gemm(const FfnArgs& a, cudaStream_t st) {
   Params p{};
   int pairs;
   AL_TRY(card_pairs(&pairs));
-  p.ksteps = (int)cdiv(a.T, BK);
+  p.ksteps = (int)cdiv(a.T, KS);
   AL_TRY(make_operand_map(&p.a[0], a.dg, a.F, a.T, a.F, 64, BK));
   AL_TRY(make_operand_map(&p.a[1], a.du, a.F, a.T, a.F, 64, BK));
   AL_TRY(make_operand_map(&p.b[0], a.x, a.H, a.T, a.ldx, 64, BK));
