@@ -200,9 +200,7 @@ int artlite_gated_ffn_backward(int dtype, int activation, const void* dh, int64_
   AL_TRY(dense_status(dev, &a.status));
   if (!dx && !dw_gate) return ARTLITE_OK;
   AL_TRY(dtype == ARTLITE_BF16 ? launch_gate_grad<__nv_bfloat16>(a, st) : launch_gate_grad<__half>(a, st));
-  if (dx) AL_TRY(launch_ffn_dx_gemm(a, st));
-  if (dw_gate) AL_TRY(launch_ffn_dw_gemm(a, st));
-  return ARTLITE_OK;
+  return launch_ffn_backward_gemm(a, st);
 }
 
 #pragma GCC visibility pop

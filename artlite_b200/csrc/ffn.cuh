@@ -25,7 +25,6 @@ struct FfnArgs {
   DevStatus* status;
 };
 int launch_ffn_forward_gemm(const FfnArgs& a, cudaStream_t st);
-int launch_ffn_dx_gemm(const FfnArgs& a, cudaStream_t st);
-int launch_ffn_dw_gemm(const FfnArgs& a, cudaStream_t st);
+int launch_ffn_backward_gemm(const FfnArgs& a, cudaStream_t st);  // dx, or dwg and dwu, or all three
 
 }  // namespace artlite

@@ -1,12 +1,14 @@
 // The gated feed-forward's products on the 5th-generation tensor cores, for a model's own 16-bit matrices (no packing:
 // they change every training step):
-//   forward  h = act(x Wg^T) (x Wu^T): both products, the activation and the product in one kernel. A tile's 256
-//            columns are 128 gate rows (CTA 0's half of B) and the 128 up rows (CTA 1's half) of the same 128 features.
-//   dx       dx = dg Wg + du Wu: one accumulator over both reductions, 2 F values deep. A is K-major (dg rows), B
-//            MN-major: the matrices as they lie (rows of H values), no transposed copy.
-//   dw       dWg = dg^T x, dWu = du^T x: the reduction is over tokens, so both operands are MN-major as they lie.
-// The transposes are the UMMA descriptors': a TMA box of 64 values x 64 k rows lands with its values consecutive, and
-// the instruction descriptor's major bits say so. Tiles past an edge read the tensor map's zeros.
+//   forward   h = act(x Wg^T) (x Wu^T): both products, the activation and the product in one kernel. A tile's 256
+//             columns are 128 gate rows (CTA 0's half of B) and the 128 up rows (CTA 1's half) of the same 128 features.
+//   backward  dx = dg Wg + du Wu (one accumulator over both reductions, 2 F values deep), dWg = dg^T x and dWu = du^T x
+//             (the reductions over tokens), all tiles of the three in one launch, the deeper ones first: the last round of
+//             one product is filled by the next one's tiles, and small products run side by side (8192 x 2048 x 8192: 391
+//             and 357 us as two launches, whose dx left 14% of its last round empty).
+// No transposed copies: dx reads the matrices, and the weights' gradients dg, du and x, as they lie, with the reduction
+// across rows. A TMA box of 64 values x 64 rows lands with its values consecutive (MN-major), and the instruction
+// descriptor's major bits say so. Tiles past an edge read the tensor map's zeros.
 //
 // Warps (192 threads): 0 TMA, 1 the MMAs (the leader CTA's), 2 - 5 the epilogue, whose results leave by TMA stores. Three
 // stages of 64 KB a CTA.
@@ -21,39 +23,64 @@ namespace {
 
 using namespace dg;
 
-enum { kForward = 0, kDx = 1, kDw = 2 };
+enum { kForward = 0, kForwardKeep = 1, kBackward = 2 };
+enum { kDx = 0, kDw = 1 };  // a backward tile's product
 constexpr int kEpilogue = 4, kThreads = 64 + 32 * kEpilogue;
 constexpr int S = 3, KS = 2 * BK, kStage = 2 * kStageBytes;  // stages, of 128 values of the reduction
 constexpr int NS = 2;                                                    // output slots a warp
 constexpr int slot_bytes(bool keep) { return keep ? kSlot : kSlot / 2; }  // (fp32 chunks; 16-bit ones)
 
-struct Params {
-  CUtensorMap a[2], b[2];  // forward: x; Wg, Wu. dx: dg, du; Wg, Wu. dw: dg, du; x
-  CUtensorMap out[2];      // forward: h. dx: dx. dw: dWg, dWu
-  CUtensorMap g, u;        // forward: the kept values
-  int rows, cols;          // of the output
-  int ksteps;              // stages a reduction (dx: of one of its two)
-  int act;
+// One product's tiles (forward and dx: of one matrix; dw: of two)
+struct Job {
   TileOrder order;
+  int rows, cols;  // of an output
+  int ksteps;      // stages a tile (dx: of one of its two reductions)
+  int tiles;       // of all its matrices
+};
+
+struct Params {
+  CUtensorMap a[2], b[2];    // forward: x; Wg, Wu. dx: dg, du; Wg, Wu
+  CUtensorMap ta[2], tb;     // dw: dg, du; x
+  CUtensorMap out[3];        // forward: h. backward: dx, dWg, dWu
+  CUtensorMap g, u;          // forward: the kept values
+  Job job[2];
+  int kind[2];               // backward: which product job i is
+  int act;
   DevStatus* status;
 };
+
+struct Tile {
+  int kind, mat, m, n;
+  const Job* job;
+};
+template <int MODE>
+__device__ __forceinline__ Tile tile_of(const Params& p, int id) {
+  Tile t;
+  const int i = MODE == kBackward && id >= p.job[0].tiles ? 1 : 0;
+  if (i) id -= p.job[0].tiles;
+  t.job = &p.job[i];
+  t.kind = p.kind[i];
+  const int per = t.job->order.tm * t.job->order.tn;
+  t.mat = MODE == kBackward && id >= per ? 1 : 0;
+  tile_at(t.job->order, id - t.mat * per, &t.m, &t.n);
+  return t;
+}
 
 struct Smem {
   uint64_t full[S], empty[S], tfull[2], tempty[2];
   uint32_t tmem_base;
   int abort;
 };
-template <bool KEEP>
+template <int MODE>
 constexpr size_t smem_bytes() {
-  return 1024 + 2 * (size_t)S * kStage + kEpilogue * NS * (size_t)slot_bytes(KEEP) + sizeof(Smem) + 64;
+  return 1024 + 2 * (size_t)S * kStage + kEpilogue * NS * (size_t)slot_bytes(MODE == kForwardKeep) + sizeof(Smem) + 64;
 }
 
-template <int MODE, class T, bool KEEP>
+template <int MODE, class T>
 __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ Params p) {
-  constexpr int SLOT = slot_bytes(KEEP);
+  constexpr bool kKeep = MODE == kForwardKeep;
+  constexpr int SLOT = slot_bytes(kKeep);
   constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
-  constexpr bool kAmn = MODE == kDw, kBmn = MODE != kForward;
-  constexpr int kMats = MODE == kDw ? 2 : 1, kSegs = MODE == kDx ? 2 : 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sA = base;
@@ -62,7 +89,8 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
   Smem* sm = reinterpret_cast<Smem*>(sOut + kEpilogue * NS * SLOT);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t crank = tc::cluster_rank();
-  const int per = p.order.tm * p.order.tn, total = per * kMats, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int total = p.job[0].tiles + (MODE == kBackward ? p.job[1].tiles : 0);
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
   griddep_launch();
   if (threadIdx.x == 0) {
@@ -88,33 +116,32 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
     // ---------------- TMA: this CTA's halves of A and B
     int s = 0, ph = 0;
     for (int id = pair; id < total; id += pairs) {
-      int m, n;
-      const int mat = id / per;
-      tile_at(p.order, id - mat * per, &m, &n);
-      const int row = m * TILE + HALF * (int)crank;
-      for (int ks = 0; ks < kSegs * p.ksteps; ks++) {
+      const Tile t = tile_of<MODE>(p, id);
+      const bool dw = MODE == kBackward && t.kind == kDw, dx = MODE == kBackward && t.kind == kDx;
+      const int ksteps = t.job->ksteps, row = t.m * TILE + HALF * (int)crank;
+      const int col = MODE == kBackward ? t.n * TILE + HALF * (int)crank : t.n * HALF;
+      for (int ks = 0; ks < (dx ? 2 : 1) * ksteps; ks++) {
         if (!tc::wait(&sm->abort, &sm->empty[s], ph ^ 1, p.status, 60)) goto out;
-        if (crank == 0)
-          tc::mbar_expect_tx(&sm->full[s], 4 * kStage);
+        if (crank == 0) tc::mbar_expect_tx(&sm->full[s], 4 * kStage);
         const uint32_t bar = tc::peer_addr(&sm->full[s], 0);
-        const int seg = kSegs == 2 && ks >= p.ksteps ? 1 : 0;
+        const int seg = dx && ks >= ksteps ? 1 : 0;
         for (int h = 0; h < 2; h++) {
-          const int k = (ks - seg * p.ksteps) * KS + h * BK;
+          const int k = (ks - seg * ksteps) * KS + h * BK;
           uint8_t *da = sA + s * kStage + h * kStageBytes, *db = sB + s * kStage + h * kStageBytes;
-          if constexpr (MODE == kForward) {
+          if (MODE != kBackward) {
             tc::tma_load_2d_pair(da, &p.a[0], bar, k, row);
-            tc::tma_load_2d_pair(db, &p.b[crank], bar, k, n * HALF);
-          } else {
-            const int col = n * TILE + HALF * (int)crank;
-            if constexpr (MODE == kDx) {
-              tc::tma_load_2d_pair(da, &p.a[seg], bar, k, row);
-            } else {
-              tc::tma_load_2d_pair(da, &p.a[mat], bar, row, k);
-              tc::tma_load_2d_pair(da + kStageBytes / 2, &p.a[mat], bar, row + 64, k);
-            }
-            tc::tma_load_2d_pair(db, &p.b[seg], bar, col, k);
-            tc::tma_load_2d_pair(db + kStageBytes / 2, &p.b[seg], bar, col + 64, k);
+            tc::tma_load_2d_pair(db, &p.b[crank], bar, k, col);
+            continue;
           }
+          const CUtensorMap* mb = dw ? &p.tb : &p.b[seg];
+          if (dw) {
+            tc::tma_load_2d_pair(da, &p.ta[t.mat], bar, row, k);
+            tc::tma_load_2d_pair(da + kStageBytes / 2, &p.ta[t.mat], bar, row + 64, k);
+          } else {
+            tc::tma_load_2d_pair(da, &p.a[seg], bar, k, row);
+          }
+          tc::tma_load_2d_pair(db, mb, bar, col, k);
+          tc::tma_load_2d_pair(db + kStageBytes / 2, mb, bar, col + 64, k);
         }
         if (++s == S) s = 0, ph ^= 1;
       }
@@ -122,23 +149,26 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
   } else if (warp == 1 && lane == 0 && crank == 0) {
     // ---------------- the MMAs
     int s = 0, ph = 0, acc = 0, aph = 0;
-    const uint32_t id_mma = tc::idesc_of(kBf16, kAmn, kBmn, TILE, TILE);
-    // a K step of 16: 32 bytes along a K-major row, 16 rows of 128 bytes of an MN-major box
-    constexpr uint64_t kStepA = kAmn ? 2048 >> 4 : 32 >> 4, kStepB = kBmn ? 2048 >> 4 : 32 >> 4;
     for (int id = pair; id < total; id += pairs) {
+      const Tile t = tile_of<MODE>(p, id);
+      const bool dw = MODE == kBackward && t.kind == kDw, dx = MODE == kBackward && t.kind == kDx;
+      const uint32_t id_mma = tc::idesc_of(kBf16, dw, MODE == kBackward, TILE, TILE);
       if (!tc::wait_cluster(&sm->abort, &sm->tempty[acc], aph ^ 1, p.status, 61)) goto out;
       tc::fence_after();
       const uint32_t d = tmem + acc * TILE;
-      for (int ks = 0; ks < kSegs * p.ksteps; ks++) {
+      // a K step of 16: 32 bytes along a K-major row, 16 rows of 128 bytes of an MN-major box
+      const uint64_t step_a = dw ? 2048 >> 4 : 32 >> 4, step_b = MODE == kBackward ? 2048 >> 4 : 32 >> 4;
+      const int ksteps = (dx ? 2 : 1) * t.job->ksteps;
+      for (int ks = 0; ks < ksteps; ks++) {
         if (!tc::wait_cluster(&sm->abort, &sm->full[s], ph, p.status, 62)) goto out;
         tc::fence_after();
         const uint32_t aa = tc::smem_u32(sA + s * kStage), ab = tc::smem_u32(sB + s * kStage);
-        const uint64_t da = kAmn ? tc::sdesc_mn(aa, kStageBytes / 2) : tc::sdesc(aa);
-        const uint64_t db = kBmn ? tc::sdesc_mn(ab, kStageBytes / 2) : tc::sdesc(ab);
+        const uint64_t da = dw ? tc::sdesc_mn(aa, kStageBytes / 2) : tc::sdesc(aa);
+        const uint64_t db = MODE == kBackward ? tc::sdesc_mn(ab, kStageBytes / 2) : tc::sdesc(ab);
 #pragma unroll
         for (int k = 0; k < KS / 16; k++) {
           const uint64_t box = (k / 4) * (kStageBytes >> 4);
-          tc::mma_pair(d, da + box + (k % 4) * kStepA, db + box + (k % 4) * kStepB, id_mma, (ks | k) != 0);
+          tc::mma_pair(d, da + box + (k % 4) * step_a, db + box + (k % 4) * step_b, id_mma, (ks | k) != 0);
         }
         tc::commit_pair(&sm->empty[s]);
         if (++s == S) s = 0, ph ^= 1;
@@ -153,26 +183,25 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
     uint8_t* mine = sOut + (warp - 2) * NS * SLOT;
     const uint32_t tempty0 = tc::peer_addr(&sm->tempty[0], 0);
     for (int id = pair; id < total; id += pairs) {
-      int m, n;
-      const int mat = id / per;
-      tile_at(p.order, id - mat * per, &m, &n);
+      const Tile t = tile_of<MODE>(p, id);
       if (!tc::wait(&sm->abort, &sm->tfull[acc], aph, p.status, 63)) goto out;
       tc::fence_after();
       const uint32_t col0 = tmem + ((uint32_t)(32 * q) << 16) + acc * TILE;
-      const int row = m * TILE + HALF * (int)crank + 32 * q;
-      constexpr int cols = MODE == kForward ? HALF : TILE;
+      const int row = t.m * TILE + HALF * (int)crank + 32 * q;
+      const CUtensorMap* out_map = &p.out[MODE == kBackward && t.kind == kDw ? 1 + t.mat : 0];
+      constexpr int cols = MODE == kBackward ? TILE : HALF;
       for (int c = 0; c < cols; c += 32) {
-        const int f = n * cols + c;
-        if (f >= p.cols || row >= p.rows) break;  // (uniform: nothing of the box is inside)
+        const int f = t.n * cols + c;
+        if (f >= t.job->cols || row >= t.job->rows) break;  // (uniform: nothing of the box is inside)
         uint32_t v[32];
         float o[32];
         tc::tmem_ld32(col0 + c, v);
-        if constexpr (MODE == kForward) {
+        if constexpr (MODE != kBackward) {
           uint32_t w[32];
           tc::tmem_ld32(col0 + HALF + c, w);
           tc::tmem_wait32(v);
           tc::tmem_wait32(w);
-          if constexpr (KEEP) {
+          if constexpr (kKeep) {
             store_wait<NS - 1>(lane);
             store_chunk<float>(mine + slot * SLOT, &p.g, f, row, reinterpret_cast<const float(&)[32]>(v), lane);
             slot = (slot + 1) & (NS - 1);
@@ -189,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
           for (int j = 0; j < 32; j++) o[j] = __uint_as_float(v[j]);
         }
         store_wait<NS - 1>(lane);
-        store_chunk<T>(mine + slot * SLOT, &p.out[mat], f, row, o, lane);
+        store_chunk<T>(mine + slot * SLOT, out_map, f, row, o, lane);
         slot = (slot + 1) & (NS - 1);
       }
       tc::fence_before();
@@ -217,20 +246,24 @@ out:
   }
 }
 
-template <int MODE, bool KEEP = false>
-int go(const Params& p, int dtype, int mats, int pairs, cudaStream_t st) {
-  const int64_t total = (int64_t)p.order.tm * p.order.tn * mats;
-  AL_CHECK(total < (1ll << 31), ARTLITE_EUNSUPPORTED, "gated_ffn: %lld tiles", (long long)total);
-  const int n = total < pairs ? (int)total : pairs;
-  return dtype == ARTLITE_BF16 ? launch_pairs(ffn_gemm<MODE, __nv_bfloat16, KEEP>, p, n, kThreads, smem_bytes<KEEP>(), st)
-                               : launch_pairs(ffn_gemm<MODE, __half, KEEP>, p, n, kThreads, smem_bytes<KEEP>(), st);
-}
-
-int card_pairs(int* out) {
+template <int MODE>
+int go(const Params& p, int dtype, cudaStream_t st) {
   int dev, sms;
   AL_CUDA(cudaGetDevice(&dev));
   AL_TRY(sm_count(dev, &sms));
-  *out = sms / 2;
+  const int total = p.job[0].tiles + p.job[1].tiles, pairs = total < sms / 2 ? total : sms / 2;
+  return dtype == ARTLITE_BF16 ? launch_pairs(ffn_gemm<MODE, __nv_bfloat16>, p, pairs, kThreads, smem_bytes<MODE>(), st)
+                               : launch_pairs(ffn_gemm<MODE, __half>, p, pairs, kThreads, smem_bytes<MODE>(), st);
+}
+
+int job_of(Job* j, int64_t rows, int64_t cols, int64_t depth, int width, int mats) {
+  j->order = {(int)cdiv(rows, TILE), (int)cdiv(cols, width)};
+  j->rows = (int)rows;
+  j->cols = (int)cols;
+  j->ksteps = (int)cdiv(depth, KS);
+  const int64_t tiles = (int64_t)j->order.tm * j->order.tn * mats;
+  AL_CHECK(tiles < (1 << 30), ARTLITE_EUNSUPPORTED, "gated_ffn: %lld tiles", (long long)tiles);
+  j->tiles = (int)tiles;
   return ARTLITE_OK;
 }
 
@@ -238,9 +271,7 @@ int card_pairs(int* out) {
 
 int launch_ffn_forward_gemm(const FfnArgs& a, cudaStream_t st) {
   Params p{};
-  int pairs;
-  AL_TRY(card_pairs(&pairs));
-  p.ksteps = (int)cdiv(a.H, KS);
+  AL_TRY(job_of(&p.job[0], a.T, a.F, a.H, HALF, 1));
   AL_TRY(make_operand_map(&p.a[0], a.x, a.H, a.T, a.ldx, BK, HALF));
   AL_TRY(make_operand_map(&p.b[0], a.wg, a.H, a.F, a.H, BK, HALF));
   AL_TRY(make_operand_map(&p.b[1], a.wu, a.H, a.F, a.H, BK, HALF));
@@ -249,46 +280,38 @@ int launch_ffn_forward_gemm(const FfnArgs& a, cudaStream_t st) {
     AL_TRY(make_tile_map(&p.g, a.g, true, a.F, a.T, a.F, 32, 32));
     AL_TRY(make_tile_map(&p.u, a.u, true, a.F, a.T, a.F, 32, 32));
   }
-  p.rows = (int)a.T;
-  p.cols = a.F;
   p.act = a.act;
-  p.order = {(int)cdiv(a.T, TILE), (int)cdiv(a.F, HALF)};
   p.status = a.status;
-  return a.g ? go<kForward, true>(p, a.dtype, 1, pairs, st) : go<kForward>(p, a.dtype, 1, pairs, st);
+  return a.g ? go<kForwardKeep>(p, a.dtype, st) : go<kForward>(p, a.dtype, st);
 }
 
-int launch_ffn_dx_gemm(const FfnArgs& a, cudaStream_t st) {
+int launch_ffn_backward_gemm(const FfnArgs& a, cudaStream_t st) {
   Params p{};
-  int pairs;
-  AL_TRY(card_pairs(&pairs));
-  p.ksteps = (int)cdiv(a.F, KS);
-  AL_TRY(make_operand_map(&p.a[0], a.dg, a.F, a.T, a.F, BK, HALF));
-  AL_TRY(make_operand_map(&p.a[1], a.du, a.F, a.T, a.F, BK, HALF));
-  AL_TRY(make_operand_map(&p.b[0], a.wg, a.H, a.F, a.H, 64, BK));
-  AL_TRY(make_operand_map(&p.b[1], a.wu, a.H, a.F, a.H, 64, BK));
-  AL_TRY(make_operand_map(&p.out[0], a.dx, a.H, a.T, a.lddx, 32, 32));
-  p.rows = (int)a.T;
-  p.cols = a.H;
-  p.order = {(int)cdiv(a.T, TILE), (int)cdiv(a.H, TILE)};
+  Job dx{}, dw{};
+  if (a.dx) {
+    AL_TRY(job_of(&dx, a.T, a.H, a.F, TILE, 1));
+    AL_TRY(make_operand_map(&p.a[0], a.dg, a.F, a.T, a.F, BK, HALF));
+    AL_TRY(make_operand_map(&p.a[1], a.du, a.F, a.T, a.F, BK, HALF));
+    AL_TRY(make_operand_map(&p.b[0], a.wg, a.H, a.F, a.H, 64, BK));
+    AL_TRY(make_operand_map(&p.b[1], a.wu, a.H, a.F, a.H, 64, BK));
+    AL_TRY(make_operand_map(&p.out[0], a.dx, a.H, a.T, a.lddx, 32, 32));
+  }
+  if (a.dwg) {
+    AL_TRY(job_of(&dw, a.F, a.H, a.T, TILE, 2));
+    AL_TRY(make_operand_map(&p.ta[0], a.dg, a.F, a.T, a.F, 64, BK));
+    AL_TRY(make_operand_map(&p.ta[1], a.du, a.F, a.T, a.F, 64, BK));
+    AL_TRY(make_operand_map(&p.tb, a.x, a.H, a.T, a.ldx, 64, BK));
+    AL_TRY(make_operand_map(&p.out[1], a.dwg, a.H, a.F, a.H, 32, 32));
+    AL_TRY(make_operand_map(&p.out[2], a.dwu, a.H, a.F, a.H, 32, 32));
+  }
+  // the deeper tiles first: a round of shallow ones ends the launch more evenly
+  const bool dw_first = dw.ksteps > 2 * dx.ksteps;
+  p.job[0] = dw_first ? dw : dx;
+  p.job[1] = dw_first ? dx : dw;
+  p.kind[0] = dw_first ? kDw : kDx;
+  p.kind[1] = dw_first ? kDx : kDw;
   p.status = a.status;
-  return go<kDx>(p, a.dtype, 1, pairs, st);
-}
-
-int launch_ffn_dw_gemm(const FfnArgs& a, cudaStream_t st) {
-  Params p{};
-  int pairs;
-  AL_TRY(card_pairs(&pairs));
-  p.ksteps = (int)cdiv(a.T, KS);
-  AL_TRY(make_operand_map(&p.a[0], a.dg, a.F, a.T, a.F, 64, BK));
-  AL_TRY(make_operand_map(&p.a[1], a.du, a.F, a.T, a.F, 64, BK));
-  AL_TRY(make_operand_map(&p.b[0], a.x, a.H, a.T, a.ldx, 64, BK));
-  AL_TRY(make_operand_map(&p.out[0], a.dwg, a.H, a.F, a.H, 32, 32));
-  AL_TRY(make_operand_map(&p.out[1], a.dwu, a.H, a.F, a.H, 32, 32));
-  p.rows = a.F;
-  p.cols = a.H;
-  p.order = {(int)cdiv(a.F, TILE), (int)cdiv(a.H, TILE)};
-  p.status = a.status;
-  return go<kDw>(p, a.dtype, 2, pairs, st);
+  return go<kBackward>(p, a.dtype, st);
 }
 
 }  // namespace artlite

@@ -494,65 +494,85 @@ template <class XT, int NT>
 __device__ void stage_digits(const Args& a, int64_t tok0, int cols, int it0, int it1, uint8_t* xs, float* sums, float* scale,
                              uint32_t* top) {
   const int units = (it1 - it0) * kUnits, total = units * NT * 8;
-  if (threadIdx.x < NT) top[threadIdx.x] = 0;
-  __syncthreads();
-  for (int pass = 0; pass < 2; pass++) {
-    for (int b = 0; b < total; b += kThreads) {
-      const int i = b + (int)threadIdx.x, t = i & 3, j = (i >> 2) & 1, n = (i >> 3) % NT, u = (i >> 3) / NT;
-      const int k = 64 * (it0 * kUnits + u) + 32 * j + 8 * t;
-      float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (i < total && n < cols && k < a.K) values8<XT>(static_cast<const XT*>(a.x) + (tok0 + n) * a.ldx, k, a.vec != 0, v);
-      if (pass == 0) {  // the largest magnitude: as bits, an infinity or NaN is above every number
-        uint32_t m = 0;
+  const int t = threadIdx.x & 3, j = (threadIdx.x >> 2) & 1;  // (kThreads is a multiple of 8)
+  auto load = [&](int i, float (&v)[8]) {
+    const int n = (i >> 3) % NT, u = (i >> 3) / NT, k = 64 * (it0 * kUnits + u) + 32 * j + 8 * t;
 #pragma unroll
-        for (int e = 0; e < 8; e++) m = max(m, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+    for (int e = 0; e < 8; e++) v[e] = 0.0f;
+    if (i < total && n < cols && k < a.K) values8<XT>(static_cast<const XT*>(a.x) + (tok0 + n) * a.ldx, k, a.vec != 0, v);
+  };
+  float held[8];  // the thread's first values stay in registers between the two passes
+  load(threadIdx.x, held);
+  for (int i = threadIdx.x; i - (int)threadIdx.x < total; i += kThreads) {
+    // the largest magnitude: as bits, an infinity or NaN is above every number
+    float v[8];
+    if (i == (int)threadIdx.x) {
 #pragma unroll
-        for (int o = 1; o < (NT == 1 ? 32 : 8); o <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-        if ((threadIdx.x & (NT == 1 ? 31 : 7)) == 0 && i < total) atomicMax(top + n, m);
-      } else {
-        const uint32_t m = top[n];
-        const bool finite = m < 0x7F800000u;
-        const int e2 = m >= 0x00800000u ? (int)(m >> 23) - 127 : -127;  // (subnormals: a little less than 2^29)
-        const int kk = m == 0 || !finite ? 0 : 29 - e2;
-        const float f0 = pow2(kk / 2), f1 = pow2(kk - kk / 2);
-        if (u == 0 && j == 0 && t == 0 && i < total) {
-          const int q = 24 - kk;
-          scale[2 * n] = finite ? pow2(q / 2) : __int_as_float(0x7FC00000);
-          scale[2 * n + 1] = pow2(q - q / 2);
-        }
-        float s = 0.0f;
-        int xi[8], hi[4];
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          s += v[e];
-          xi[e] = finite ? __float2int_rn(v[e] * f0 * f1) : 0;
-        }
-        s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
-        s += __shfl_xor_sync(0xFFFFFFFFu, s, 2);
-        // byte m holds values 4 m (mod 8) + m / 2 (low nibble) and the one two further (high nibble)
-        uint32_t raw[4], low[4];
-#pragma unroll
-        for (int b4 = 0; b4 < 4; b4++) {
-          const int lo = ((4 * b4) & 7) + (b4 >> 1);
-          hi[b4] = (xi[lo + 2] + 8) >> 4;
-          raw[b4] = (uint32_t)hi[b4] + 0x80808080u;  // (digits + 128 in the bytes)
-          low[b4] = (uint32_t)(xi[lo] - hi[b4]) + 0x80808080u;
-        }
-        if (i < total) {
-#pragma unroll
-          for (int p = 0; p < 4; p++) {
-            const uint32_t sel = (uint32_t)(3 - p) | (uint32_t)(7 - p) << 4;
-            const uint32_t r = __byte_perm(__byte_perm(raw[0], raw[1], sel), __byte_perm(raw[2], raw[3], sel), 0x5410);
-            const uint32_t l = __byte_perm(__byte_perm(low[0], low[1], sel), __byte_perm(low[2], low[3], sel), 0x5410);
-            reinterpret_cast<uint2*>(xs)[(u * NT + n) * 32 + (4 * j + p) * 4 + t] =
-                make_uint2(r ^ 0x80808080u, l ^ 0x80808080u);
-          }
-          // lanes t = 2 j and 2 j + 1 belong to group j
-          if (t < 2) sums[(u * NT + n) * 4 + 2 * j + t] = t == 0 ? s : 0.0f;
-        }
-      }
+      for (int e = 0; e < 8; e++) v[e] = held[e];
+    } else {
+      load(i, v);
     }
-    __syncthreads();
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) m = max(m, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+    if constexpr (NT == 1) {
+      m = __reduce_max_sync(0xFFFFFFFFu, m);
+      if ((threadIdx.x & 31) == 0) atomicMax(top, m);
+    } else {
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+      if ((threadIdx.x & 7) == 0 && i < total) atomicMax(top + (i >> 3) % NT, m);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i - (int)threadIdx.x < total; i += kThreads) {
+    const int n = (i >> 3) % NT, u = (i >> 3) / NT;
+    float v[8];
+    if (i == (int)threadIdx.x) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] = held[e];
+    } else {
+      load(i, v);
+    }
+    const uint32_t m = top[n];
+    const bool finite = m < 0x7F800000u;
+    const int e2 = m >= 0x00800000u ? (int)(m >> 23) - 127 : -127;  // (subnormals: a little less than 2^29)
+    const int kk = m == 0 || !finite ? 0 : 29 - e2;
+    const float f0 = pow2(kk / 2), f1 = pow2(kk - kk / 2);
+    if (u == 0 && j == 0 && t == 0 && i < total) {
+      const int q = 24 - kk;
+      scale[2 * n] = finite ? pow2(q / 2) : __int_as_float(0x7FC00000);
+      scale[2 * n + 1] = pow2(q - q / 2);
+    }
+    float s = 0.0f;
+    int xi[8], hi[4];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      s += v[e];
+      xi[e] = finite ? __float2int_rn(v[e] * f0 * f1) : 0;
+    }
+    s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
+    s += __shfl_xor_sync(0xFFFFFFFFu, s, 2);
+    // byte m holds values 4 m (mod 8) + m / 2 (low nibble) and the one two further (high nibble)
+    uint32_t raw[4], low[4];
+#pragma unroll
+    for (int b4 = 0; b4 < 4; b4++) {
+      const int lo = ((4 * b4) & 7) + (b4 >> 1);
+      hi[b4] = (xi[lo + 2] + 8) >> 4;
+      raw[b4] = (uint32_t)hi[b4] + 0x80808080u;  // (digits + 128 in the bytes)
+      low[b4] = (uint32_t)(xi[lo] - hi[b4]) + 0x80808080u;
+    }
+    if (i < total) {
+#pragma unroll
+      for (int p = 0; p < 4; p++) {
+        const uint32_t sel = (uint32_t)(3 - p) | (uint32_t)(7 - p) << 4;
+        const uint32_t r = __byte_perm(__byte_perm(raw[0], raw[1], sel), __byte_perm(raw[2], raw[3], sel), 0x5410);
+        const uint32_t l = __byte_perm(__byte_perm(low[0], low[1], sel), __byte_perm(low[2], low[3], sel), 0x5410);
+        reinterpret_cast<uint2*>(xs)[(u * NT + n) * 32 + (4 * j + p) * 4 + t] = make_uint2(r ^ 0x80808080u, l ^ 0x80808080u);
+      }
+      // lanes t = 2 j and 2 j + 1 belong to group j
+      if (t < 2) sums[(u * NT + n) * 4 + 2 * j + t] = t == 0 ? s : 0.0f;
+    }
   }
 }
 
@@ -594,7 +614,10 @@ __global__ void __launch_bounds__(kThreads, 1) small_batch(const __grid_constant
   const bool works = tl < tp && it0 + kl < it1;
 
   griddep_launch();
+  float* scale = reinterpret_cast<float*>(abort + 2);
+  uint32_t* top = reinterpret_cast<uint32_t*>(scale + 8);
   if (threadIdx.x == 0) *abort = 0;
+  if (S::kInt && threadIdx.x < NT) top[threadIdx.x] = 0;
   if (lane == 0) {
     for (int i = 0; i < a.plan.depth; i++) tc::mbar_init(full + i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -614,6 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1) small_batch(const __grid_constant
   if constexpr (S::kPlain) griddep_wait();
   if (works && lane == 0)
     for (int i = 0; i < a.plan.depth; i++) request(i);
+  if constexpr (S::kInt) __syncthreads();
   if constexpr (!S::kPlain) griddep_wait();
 
   const uint32_t* table = nullptr;
@@ -622,31 +646,40 @@ __global__ void __launch_bounds__(kThreads, 1) small_batch(const __grid_constant
     for (int i = threadIdx.x; i < 256 * 32; i += kThreads) tb[i] = iq4_pair<B>(i >> 5);
     table = tb + lane;
   }
-  float* scale = reinterpret_cast<float*>(abort + 2);
   if constexpr (S::kInt) {
-    stage_digits<XT, NT>(a, tok0, cols, it0, it1, sm + a.plan.x_off, reinterpret_cast<float*>(sm + a.plan.sum_off), scale,
-                         reinterpret_cast<uint32_t*>(scale + 8));
+    stage_digits<XT, NT>(a, tok0, cols, it0, it1, sm + a.plan.x_off, reinterpret_cast<float*>(sm + a.plan.sum_off), scale, top);
   } else {  // x: [unit][plane][half j][column][t] 16 B, and [unit][half][column] the sums of a group's 32 values
     constexpr int kUnitsItem = S::kItemK / 64;
     const int units = (it1 - it0) * kUnitsItem, total = units * 2 * cols * 4;
     float* sums = reinterpret_cast<float*>(sm + a.plan.sum_off);
-    for (int b = 0; b < total; b += kThreads) {
-      const int i = b + (int)threadIdx.x, tt = i & 3, col = (i >> 2) % cols, uj = (i >> 2) / cols;
-      const int k = 64 * (it0 * kUnitsItem + (uj >> 1)) + (S::kPlain ? 16 * tt + 8 * (uj & 1) : 32 * (uj & 1) + 8 * tt);
-      uint4 f[P];
+    // (some loads at a time: a load's way to L2 and back is longer than all the rest of a round)
+    constexpr int kAhead = sizeof(XT) == 4 ? 2 : 4;
+    for (int b = threadIdx.x; b - (int)threadIdx.x < total; b += kAhead * kThreads) {
+      uint4 f[kAhead][P];
+      float s[kAhead];
 #pragma unroll
-      for (int pl = 0; pl < P; pl++) f[pl] = make_uint4(0, 0, 0, 0);
-      float s = 0.0f;
-      if (i < total && k < a.K) s = fragment<XT>(static_cast<const XT*>(a.x) + (tok0 + col) * a.ldx, k, a.vec != 0, f);
-      if (i < total) {
+      for (int h = 0; h < kAhead; h++) {
+        const int i = b + h * kThreads, tt = i & 3, uj = (i >> 2) / cols, col = (i >> 2) - uj * cols;
+        const int k = 64 * (it0 * kUnitsItem + (uj >> 1)) + (S::kPlain ? 16 * tt + 8 * (uj & 1) : 32 * (uj & 1) + 8 * tt);
 #pragma unroll
-        for (int pl = 0; pl < P; pl++)
-          reinterpret_cast<uint4*>(sm + a.plan.x_off)[((((uj >> 1) * P + pl) * 2 + (uj & 1)) * cols + col) * 4 + tt] = f[pl];
+        for (int pl = 0; pl < P; pl++) f[h][pl] = make_uint4(0, 0, 0, 0);
+        s[h] = 0.0f;
+        if (i < total && k < a.K) s[h] = fragment<XT>(static_cast<const XT*>(a.x) + (tok0 + col) * a.ldx, k, a.vec != 0, f[h]);
       }
-      if constexpr (S::kMin) {
-        s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
-        s += __shfl_xor_sync(0xFFFFFFFFu, s, 2);
-        if (i < total && tt == 0) sums[uj * 8 * NT + col] = s;
+#pragma unroll
+      for (int h = 0; h < kAhead; h++) {
+        const int i = b + h * kThreads, tt = i & 3, uj = (i >> 2) / cols, col = (i >> 2) - uj * cols;
+        if (i < total) {
+#pragma unroll
+          for (int pl = 0; pl < P; pl++)
+            reinterpret_cast<uint4*>(sm + a.plan.x_off)[((((uj >> 1) * P + pl) * 2 + (uj & 1)) * cols + col) * 4 + tt] = f[h][pl];
+        }
+        if constexpr (S::kMin) {
+          float v = s[h];
+          v += __shfl_xor_sync(0xFFFFFFFFu, v, 1);
+          v += __shfl_xor_sync(0xFFFFFFFFu, v, 2);
+          if (i < total && tt == 0) sums[uj * 8 * NT + col] = v;
+        }
       }
     }
   }
