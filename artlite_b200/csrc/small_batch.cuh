@@ -245,32 +245,43 @@ struct Quant {
       }
       const uint8_t* xu = x.x + (unit0 + u) * P * 128 * x.cols;
       const float* su = x.sums + (unit0 + u) * 16 * NT;
+      // (both groups side by side: independent MMAs follow one another, not a group's two)
+      uint32_t A[2][2][4];  // [group][step]
 #pragma unroll
       for (int j = 0; j < 2; j++) {
-        uint32_t a[2][4], A[2][4];
+        uint32_t a[2][4];
         unpack<B, kSub>(j ? q.z : q.x, table, a[0]);
         unpack<B, kSub>(j ? q.w : q.y, table, a[1]);
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) A[h][i] = a[i & 1][2 * h + (i >> 1)];
+          for (int i = 0; i < 4; i++) A[j][h][i] = a[i & 1][2 * h + (i >> 1)];
+      }
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-          float c[4];
+      for (int n = 0; n < NT; n++) {
+        float c[2][4];
 #pragma unroll
-          for (int pl = 0; pl < P; pl++) {
-            const uint4 b = *reinterpret_cast<const uint4*>(xu + (2 * pl + j) * 64 * x.cols + x.col[n]);
-            if (pl == 0) mma0<B>(c, A[0], b.x, b.y);
-            else mma<B>(c, A[0], b.x, b.y);
-            mma<B>(c, A[1], b.z, b.w);
+        for (int pl = 0; pl < P; pl++) {
+          uint4 b[2];
+#pragma unroll
+          for (int j = 0; j < 2; j++) b[j] = *reinterpret_cast<const uint4*>(xu + (2 * pl + j) * 64 * x.cols + x.col[n]);
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            if (pl == 0) mma0<B>(c[j], A[j][0], b[j].x, b[j].y);
+            else mma<B>(c[j], A[j][0], b[j].x, b[j].y);
           }
 #pragma unroll
-          for (int i = 0; i < 4; i++) acc.v[n][i] = fmaf(sc[i >> 1][j], c[i], acc.v[n][i]);
+          for (int j = 0; j < 2; j++) mma<B>(c[j], A[j][1], b[j].z, b[j].w);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
           if constexpr (kMin) {
             const float2 s = *reinterpret_cast<const float2*>(su + j * 8 * NT + 8 * n);
 #pragma unroll
             for (int i = 0; i < 4; i++) acc.v[n][i] = fmaf(mn[i >> 1][j], i & 1 ? s.y : s.x, acc.v[n][i]);
           }
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc.v[n][i] = fmaf(sc[i >> 1][j], c[j][i], acc.v[n][i]);
         }
       }
     }
@@ -642,9 +653,12 @@ __global__ void __launch_bounds__(kThreads, 1) small_batch(const __grid_constant
 
   const uint32_t* table = nullptr;
   if constexpr (S::kTable) {  // a copy of the table for every lane: reads without bank conflicts
-    uint32_t* tb = reinterpret_cast<uint32_t*>(sm + a.plan.table_off);
-    for (int i = threadIdx.x; i < 256 * 32; i += kThreads) tb[i] = iq4_pair<B>(i >> 5);
-    table = tb + lane;
+    uint4* tb = reinterpret_cast<uint4*>(sm + a.plan.table_off);
+    const int e = threadIdx.x >> 1;  // (half an entry's copies a thread; the order keeps eight lanes in distinct banks)
+    const uint32_t v = iq4_pair<B>(e);
+#pragma unroll
+    for (int i = 0; i < 4; i++) tb[8 * e + 4 * (threadIdx.x & 1) + ((i + e) & 3)] = make_uint4(v, v, v, v);
+    table = reinterpret_cast<const uint32_t*>(tb) + lane;
   }
   if constexpr (S::kInt) {
     stage_digits<XT, NT>(a, tok0, cols, it0, it1, sm + a.plan.x_off, reinterpret_cast<float*>(sm + a.plan.sum_off), scale, top);
