@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
   uint8_t* sB = sA + S * kStage;
   uint8_t* sOut = sB + S * kStage;
   Smem* sm = reinterpret_cast<Smem*>(sOut + kEpilogue * NS * SLOT);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = tc::warp_index(), lane = threadIdx.x & 31;
   const uint32_t crank = tc::cluster_rank();
   const int total = p.job[0].tiles + (MODE == kBackward ? p.job[1].tiles : 0);
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -146,34 +146,38 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
         if (++s == S) s = 0, ph ^= 1;
       }
     }
-  } else if (warp == 1 && lane == 0 && crank == 0) {
+  } else if (warp == 1 && crank == 0) {
     // ---------------- the MMAs
     int s = 0, ph = 0, acc = 0, aph = 0;
     for (int id = pair; id < total; id += pairs) {
       const Tile t = tile_of<MODE>(p, id);
       const bool dw = MODE == kBackward && t.kind == kDw, dx = MODE == kBackward && t.kind == kDx;
       const uint32_t id_mma = tc::idesc_of(kBf16, dw, MODE == kBackward, TILE, TILE);
-      if (!tc::wait_cluster(&sm->abort, &sm->tempty[acc], aph ^ 1, p.status, 61)) goto out;
+      if (!__all_sync(0xFFFFFFFFu, tc::wait_cluster(&sm->abort, &sm->tempty[acc], aph ^ 1, p.status, 61))) goto out;
       tc::fence_after();
       const uint32_t d = tmem + acc * TILE;
       // a K step of 16: 32 bytes along a K-major row, 16 rows of 128 bytes of an MN-major box
       const uint64_t step_a = dw ? 2048 >> 4 : 32 >> 4, step_b = MODE == kBackward ? 2048 >> 4 : 32 >> 4;
       const int ksteps = (dx ? 2 : 1) * t.job->ksteps;
       for (int ks = 0; ks < ksteps; ks++) {
-        if (!tc::wait_cluster(&sm->abort, &sm->full[s], ph, p.status, 62)) goto out;
+        if (!__all_sync(0xFFFFFFFFu, tc::wait_cluster(&sm->abort, &sm->full[s], ph, p.status, 62))) goto out;
         tc::fence_after();
         const uint32_t aa = tc::smem_u32(sA + s * kStage), ab = tc::smem_u32(sB + s * kStage);
         const uint64_t da = dw ? tc::sdesc_mn(aa, kStageBytes / 2) : tc::sdesc(aa);
         const uint64_t db = MODE == kBackward ? tc::sdesc_mn(ab, kStageBytes / 2) : tc::sdesc(ab);
+        if (tc::elect_one()) {
 #pragma unroll
-        for (int k = 0; k < KS / 16; k++) {
-          const uint64_t box = (k / 4) * (kStageBytes >> 4);
-          tc::mma_pair(d, da + box + (k % 4) * step_a, db + box + (k % 4) * step_b, id_mma, (ks | k) != 0);
+          for (int k = 0; k < KS / 16; k++) {
+            const uint64_t box = (k / 4) * (kStageBytes >> 4);
+            tc::mma_pair(d, da + box + (k % 4) * step_a, db + box + (k % 4) * step_b, id_mma, (ks | k) != 0);
+          }
+          tc::commit_pair(&sm->empty[s]);
         }
-        tc::commit_pair(&sm->empty[s]);
+        __syncwarp();
         if (++s == S) s = 0, ph ^= 1;
       }
-      tc::commit_pair(&sm->tfull[acc]);
+      if (tc::elect_one()) tc::commit_pair(&sm->tfull[acc]);
+      __syncwarp();
       if (++acc == 2) acc = 0, aph ^= 1;
     }
   } else if (warp >= 2) {

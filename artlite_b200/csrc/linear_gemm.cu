@@ -29,7 +29,8 @@ using namespace dg;
 // A stage is 128 values of K (two boxes of 64): half as many hand-overs between the decoding and the MMAs as with 64.
 // Stages of A and of B, packed chunks in flight
 constexpr int KS = 2 * BK, kStage = 2 * kStageBytes;
-constexpr int SA = 3, SB = 2, R = 2;
+constexpr int SA_MAX = 6, SB_MAX = 4, R_MAX = 6;
+constexpr int kMaxSets = 2;
 constexpr int kDecodeWarps = 8, kThreads = 256 + 32 * kDecodeWarps;
 
 struct Params {
@@ -41,6 +42,8 @@ struct Params {
   const int32_t* row_exp;
   int w_exp0, w_exp1;
   int T, K, N;
+  int sa;     // stages of A
+  int width;  // columns of a tile's accumulator (gated: gate and up together): 256, 128 or 64
   int act;
   bool vec_y;
   TileOrder order;
@@ -48,15 +51,30 @@ struct Params {
 };
 
 struct Smem {
-  uint64_t full_a[SA], empty_a[SA], full_b[SB], empty_b[SB], raw_full[R], raw_empty[R], tfull[2], tempty[2];
+  uint64_t full_a[SA_MAX], empty_a[SA_MAX], full_b[SB_MAX], empty_b[SB_MAX], raw_full[R_MAX], raw_empty[R_MAX], tfull[2], tempty[2];
   uint32_t tmem_base;
   int abort;
 };
 
+// shared memory: sa stages of A, b_stages of B (width / 2 rows), raw_chunks of packed tiles; as many stages of A as fit
+#ifndef R256
+#define R256 3
+#define RN 6
+#endif
+constexpr int b_stages(int width) { return width == 256 ? 2 : SB_MAX; }  // (a multiple of the sets)
+constexpr int raw_chunks(int width) { return width == 256 ? R256 : RN; }
 template <int QT>
-constexpr size_t smem_bytes() {
-  return 1024 + (size_t)(SA + SB) * kStage + (size_t)R * 8 * tile_bytes(QT) + sizeof(Smem) +
+constexpr int fixed_bytes(int width) {
+  return 1024 + b_stages(width) * (width / 2) * KS * 2 + raw_chunks(width) * (width / 32) * tile_bytes(QT) + (int)sizeof(Smem) +
          (QT == ARTLITE_IQ4_NL ? 256 * 4 : 0) + 64;
+}
+template <int QT>
+constexpr int a_stages(int width) {
+  return (227 * 1024 - fixed_bytes<QT>(width)) / kStage < SA_MAX ? (227 * 1024 - fixed_bytes<QT>(width)) / kStage : SA_MAX;
+}
+template <int QT>
+constexpr size_t smem_bytes(int width) {
+  return (size_t)fixed_bytes<QT>(width) + (size_t)a_stages<QT>(width) * kStage;
 }
 
 __device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -135,14 +153,17 @@ __device__ __forceinline__ uint4 decode8(uint32_t w, __half2 d, __half2 m, const
 template <int QT, class T, bool GATED>
 __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant__ Params p) {
   constexpr int TB = tile_bytes(QT);
+  // a CTA's half of B: its rows, its row tiles, and the sets of warps that take the stages in turn
+  const int half = p.width / 2, row_tiles = half / kTileRows, sets = row_tiles < kDecodeWarps ? kMaxSets : 1;
+  const int SA = p.sa, SB = b_stages(p.width), R = raw_chunks(p.width), box = half * 128;  // (a box: 64 values of each of B's rows)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sA = base;
   uint8_t* sB = sA + SA * kStage;
-  uint8_t* sR = sB + SB * kStage;
-  Smem* sm = reinterpret_cast<Smem*>(sR + R * 8 * TB);
+  uint8_t* sR = sB + SB * 2 * box;
+  Smem* sm = reinterpret_cast<Smem*>(sR + R * row_tiles * TB);
   uint32_t* table = reinterpret_cast<uint32_t*>(sm + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = tc::warp_index(), lane = threadIdx.x & 31;
   const uint32_t crank = tc::cluster_rank();
   const int total = p.order.tm * p.order.tn, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int ksteps = (p.K + KS - 1) / KS, chunks = (p.K + kTileK - 1) / kTileK;
@@ -154,12 +175,12 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
       tc::mbar_init(&sm->empty_a[i], 1);
     }
     for (int i = 0; i < SB; i++) {
-      tc::mbar_init(&sm->full_b[i], 2 * kDecodeWarps);
+      tc::mbar_init(&sm->full_b[i], 2 * row_tiles);
       tc::mbar_init(&sm->empty_b[i], 1);
     }
     for (int i = 0; i < R; i++) {
       tc::mbar_init(&sm->raw_full[i], 1);
-      tc::mbar_init(&sm->raw_empty[i], kDecodeWarps);
+      tc::mbar_init(&sm->raw_empty[i], sets * row_tiles);
     }
     for (int i = 0; i < 2; i++) {
       tc::mbar_init(&sm->tfull[i], 1);
@@ -196,30 +217,34 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
         if (++s == SA) s = 0, ph ^= 1;
       }
     }
-  } else if (warp == 1 && lane == 0 && crank == 0) {
+  } else if (warp == 1 && crank == 0) {
     // ---------------- the MMAs
     int s = 0, ph = 0, b = 0, bph = 0, acc = 0, aph = 0;
-    const uint32_t id_mma = tc::idesc_of(false, false, false, TILE, TILE);
+    const uint32_t id_mma = tc::idesc_of(false, false, false, TILE, p.width);
     for (int id = pair; id < total; id += pairs) {
-      if (!tc::wait_cluster(&sm->abort, &sm->tempty[acc], aph ^ 1, p.status, 41)) goto out;
+      if (!__all_sync(0xFFFFFFFFu, tc::wait_cluster(&sm->abort, &sm->tempty[acc], aph ^ 1, p.status, 41))) goto out;
       tc::fence_after();
       const uint32_t d = tmem + acc * TILE;
       for (int ks = 0; ks < ksteps; ks++) {
-        if (!tc::wait_cluster(&sm->abort, &sm->full_a[s], ph, p.status, 42)) goto out;
-        if (!tc::wait_cluster(&sm->abort, &sm->full_b[b], bph, p.status, 43)) goto out;
+        if (!__all_sync(0xFFFFFFFFu, tc::wait_cluster(&sm->abort, &sm->full_a[s], ph, p.status, 42))) goto out;
+        if (!__all_sync(0xFFFFFFFFu, tc::wait_cluster(&sm->abort, &sm->full_b[b], bph, p.status, 43))) goto out;
         tc::fence_after();
-        const uint64_t da = tc::sdesc(tc::smem_u32(sA + s * kStage)), db = tc::sdesc(tc::smem_u32(sB + b * kStage));
+        const uint64_t da = tc::sdesc(tc::smem_u32(sA + s * kStage)), db = tc::sdesc(tc::smem_u32(sB + b * 2 * box));
+        if (tc::elect_one()) {
 #pragma unroll
-        for (int k = 0; k < KS / 16; k++) {
-          const uint64_t at = (k / 4) * (kStageBytes >> 4) + 2 * (k % 4);
-          tc::mma_pair(d, da + at, db + at, id_mma, (ks | k) != 0);
+          for (int k = 0; k < KS / 16; k++) {
+            tc::mma_pair(d, da + (k / 4) * (kStageBytes >> 4) + 2 * (k % 4), db + (k / 4) * (box >> 4) + 2 * (k % 4), id_mma,
+                         (ks | k) != 0);
+          }
+          tc::commit_pair(&sm->empty_a[s]);
+          tc::commit_pair(&sm->empty_b[b]);
         }
-        tc::commit_pair(&sm->empty_a[s]);
-        tc::commit_pair(&sm->empty_b[b]);
+        __syncwarp();
         if (++s == SA) s = 0, ph ^= 1;
         if (++b == SB) b = 0, bph ^= 1;
       }
-      tc::commit_pair(&sm->tfull[acc]);
+      if (tc::elect_one()) tc::commit_pair(&sm->tfull[acc]);
+      __syncwarp();
       if (++acc == 2) acc = 0, aph ^= 1;
     }
   } else if (warp == 2 && lane == 0) {
@@ -229,14 +254,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
       int m, n;
       tile_at(p.order, id, &m, &n);
       const uint8_t* w = GATED ? p.w[crank] : p.w[0];
-      const int64_t mt0 = GATED ? 8 * (int64_t)n : 16 * (int64_t)n + 8 * crank;
+      const int64_t mt0 = (GATED ? n : 2 * (int64_t)n + crank) * row_tiles;
       // (past the matrix: its last rows again, whose products no output reads)
-      const int64_t mt = min64(mt0, p.row_tiles - 8);
+      const int64_t mt = min64(mt0, p.row_tiles - row_tiles);
       for (int ch = 0; ch < chunks; ch++) {
         if (!tc::wait(&sm->abort, &sm->raw_empty[r], rph ^ 1, p.status, 44)) goto out;
-        tc::mbar_expect_tx(&sm->raw_full[r], 8 * TB);
-        for (int i = 0; i < 8; i++)
-          bulk_copy(sR + (r * 8 + i) * TB, w + ((mt + i) * chunks + ch) * TB, TB, &sm->raw_full[r]);
+        tc::mbar_expect_tx(&sm->raw_full[r], row_tiles * TB);
+        for (int i = 0; i < row_tiles; i++)
+          bulk_copy(sR + (r * row_tiles + i) * TB, w + ((mt + i) * chunks + ch) * TB, TB, &sm->raw_full[r]);
         if (++r == R) r = 0, rph ^= 1;
       }
     }
@@ -244,7 +269,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
     // ---------------- the decoding: warp 8 + i turns row tile i of every stage into fp16 rows of B (K-major, 128-byte
     // swizzle: 16-byte chunk c of row i at chunk c ^ (i & 7))
     // Odd rows take their two groups in the other order: eight lanes' 16-byte stores then fall in distinct banks
-    const int i = warp - 8, g = lane >> 2, t = lane & 3, odd = g & 1;
+    const int set = (warp - 8) / row_tiles, i = (warp - 8) - set * row_tiles, g = lane >> 2, t = lane & 3, odd = g & 1;
+    if (set >= sets) goto out;
     int s = 0, ph = 0, r = 0, rph = 0;
     const uint32_t full_b0 = tc::peer_addr(&sm->full_b[0], 0);
     const int we = GATED && crank ? p.w_exp1 : p.w_exp0;
@@ -253,18 +279,29 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
     for (int id = pair; id < total; id += pairs) {
       for (int ch = 0; ch < chunks; ch++) {
         if (!tc::wait(&sm->abort, &sm->raw_full[r], rph, p.status, 45)) goto out;
-        const uint8_t* tile = sR + (r * 8 + i) * TB;
+        const uint8_t* tile = sR + (r * row_tiles + i) * TB;
         const int stages = min(kUnits / 2, ksteps - kUnits / 2 * ch);
+        // the chunk's codes and scales into registers, and its place to the next chunk
+        uint4 q[kUnits];
+#pragma unroll
+        for (int u = 0; u < kUnits; u++) q[u] = reinterpret_cast<const uint4*>(tile)[32 * u + lane];
         sc.load(tile, g);
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&sm->raw_empty[r]);
+        if (++r == R) r = 0, rph ^= 1;
 #pragma unroll
         for (int h = 0; h < kUnits / 2; h++) {
           if (h >= stages) break;
+          if ((s & (sets - 1)) != set) {  // (the other set's)
+            if (++s == SB) s = 0, ph ^= 1;
+            continue;
+          }
           // [unit of the stage][row][group, the lane's first and second]: word 2 j + row of the lane's codes
           uint4 c[2][2][2];
 #pragma unroll
           for (int v = 0; v < 2; v++) {
-            const uint4 q = reinterpret_cast<const uint4*>(tile)[32 * (2 * h + v) + lane];
-            const uint32_t w[2][2] = {{odd ? q.z : q.x, odd ? q.x : q.z}, {odd ? q.w : q.y, odd ? q.y : q.w}};
+            const uint4 w4 = q[2 * h + v];
+            const uint32_t w[2][2] = {{odd ? w4.z : w4.x, odd ? w4.x : w4.z}, {odd ? w4.w : w4.y, odd ? w4.y : w4.w}};
 #pragma unroll
             for (int jj = 0; jj < 2; jj++) {
               __half2 d, m;
@@ -274,14 +311,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
             }
           }
           if (!tc::wait(&sm->abort, &sm->empty_b[s], ph ^ 1, p.status, 46)) goto out;
-          uint8_t* row = sB + s * kStage + (16 * i + g) * 128;
+          uint8_t* row = sB + s * 2 * box + (16 * i + g) * 128;
 #pragma unroll
           for (int v = 0; v < 2; v++)
 #pragma unroll
             for (int rr = 0; rr < 2; rr++)
 #pragma unroll
               for (int jj = 0; jj < 2; jj++)
-                *reinterpret_cast<uint4*>(row + v * kStageBytes + rr * 1024 + (((4 * (jj ^ odd) + t) ^ g) << 4)) = c[v][rr][jj];
+                *reinterpret_cast<uint4*>(row + v * box + rr * 1024 + (((4 * (jj ^ odd) + t) ^ g) << 4)) = c[v][rr][jj];
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
@@ -290,9 +327,6 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
           }
           if (++s == SB) s = 0, ph ^= 1;
         }
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sm->raw_empty[r]);
-        if (++r == R) r = 0, rph ^= 1;
       }
     }
   } else if (warp >= 4) {
@@ -314,15 +348,15 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
       const float a0 = pow2(e0 / 2), a1 = pow2(e0 - e0 / 2);
       const float b0 = pow2(e1 / 2), b1 = pow2(e1 - e1 / 2);
       T* row = static_cast<T*>(p.y) + (int64_t)tok * p.ldy;
-      constexpr int kCols = GATED ? HALF : TILE;
-      for (int c = 0; c < kCols; c += 16) {
-        const int f = n * kCols + c;
+      const int cols = GATED ? half : p.width;
+      for (int c = 0; c < cols; c += 16) {
+        const int f = n * cols + c;
         uint32_t v[16];
         float o[16];
         tc::tmem_ld16(col0 + c, v);
         if constexpr (GATED) {
           uint32_t w[16];
-          tc::tmem_ld16(col0 + HALF + c, w);
+          tc::tmem_ld16(col0 + half + c, w);
           tc::tmem_wait16(v);
           tc::tmem_wait16(w);
 #pragma unroll
@@ -360,12 +394,13 @@ out:
 }
 
 template <int QT, class T, bool GATED>
-int go(const Params& p, cudaStream_t st) {
+int go(Params p, cudaStream_t st) {
+  p.sa = a_stages<QT>(p.width);
   int dev, sms;
   AL_CUDA(cudaGetDevice(&dev));
   AL_TRY(sm_count(dev, &sms));
   const int total = p.order.tm * p.order.tn;
-  return launch_pairs(linear_gemm<QT, T, GATED>, p, total < sms / 2 ? total : sms / 2, kThreads, smem_bytes<QT>(), st);
+  return launch_pairs(linear_gemm<QT, T, GATED>, p, total < sms / 2 ? total : sms / 2, kThreads, smem_bytes<QT>(p.width), st);
 }
 template <int QT>
 int go_of(const Params& p, bool gated, bool bf16, cudaStream_t st) {
@@ -408,6 +443,20 @@ int make_tile_map(CUtensorMap* m, const void* base, bool f32, int64_t cols, int6
 
 }  // namespace dg
 
+// The width of a tile: rounds of tiles over the card's pairs times a stage's cycles. Few tokens give few tiles, and narrow
+// ones then keep more of the SMs at work; wide ones read a token row less often and decode for more MMAs. Cycles a stage
+// from measured launches (64: A's copies, 128: the MMAs and copies, 256: the MMAs and the decoding).
+int width_for(int64_t tm, int64_t N, int per, int pairs) {
+  constexpr int kWidth[] = {256, 128, 64}, kCycles[] = {1250, 750, 600};
+  int best = 256;
+  int64_t best_cost = -1;
+  for (int i = 0; i < 3; i++) {
+    const int64_t cost = cdiv(tm * cdiv(N, kWidth[i] / per), pairs) * kCycles[i];
+    if (best_cost < 0 || cost < best_cost) best = kWidth[i], best_cost = cost;
+  }
+  return best;
+}
+
 int launch_linear_gemm(const LinearGemmArgs& a, cudaStream_t st) {
   Params p{};
   AL_TRY(make_operand_map(&p.map_x, a.x, a.K, a.T, a.ldx, BK, HALF));
@@ -425,7 +474,11 @@ int launch_linear_gemm(const LinearGemmArgs& a, cudaStream_t st) {
   p.act = a.act;
   p.vec_y = ((uintptr_t)a.y % 16) == 0 && a.ldy % 8 == 0;
   p.order.tm = (int)cdiv(a.T, TILE);
-  p.order.tn = (int)cdiv(a.N, a.gated ? HALF : TILE);
+  int dev, sms;
+  AL_CUDA(cudaGetDevice(&dev));
+  AL_TRY(sm_count(dev, &sms));
+  p.width = width_for(p.order.tm, a.N, a.gated ? 2 : 1, sms / 2);
+  p.order.tn = (int)cdiv(a.N, p.width / (a.gated ? 2 : 1));
   p.status = a.status;
   AL_CHECK((int64_t)p.order.tm * p.order.tn < (1ll << 31), ARTLITE_EUNSUPPORTED, "linear: T %lld by %d rows", (long long)a.T, a.N);
   const bool bf16 = a.out_dtype == ARTLITE_BF16;

@@ -48,6 +48,17 @@ __device__ __forceinline__ bool wait(int* abort, uint64_t* bar, uint32_t parity,
   }
 }
 
+// one lane of a converged warp. A warp that runs the MMA loop whole and issues by its elected lane keeps addresses and
+// descriptors in uniform registers, where the MMAs take them from; a loop run by lane 0 alone moved them there for every
+// MMA (eight MMAs and two commits 660 - 990 cycles)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+// the warp's index, the same for the compiler in every lane
+__device__ __forceinline__ int warp_index() { return __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0); }
+
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
