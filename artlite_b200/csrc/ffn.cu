@@ -144,7 +144,9 @@ int artlite_gated_ffn(int dtype, int activation, const void* x, int64_t ldx, con
   a.H = n_in;
   a.F = n_ffn;
   AL_TRY(dense_status(dev, &a.status));
-  return forward(a, dev, static_cast<cudaStream_t>(stream));
+  const int rc = forward(a, dev, static_cast<cudaStream_t>(stream));
+  if (rc == ARTLITE_ECUDA) cudaGetLastError();  // (reported here, not by the next launch)
+  return rc;
 }
 
 int artlite_gated_ffn_backward(int dtype, int activation, const void* dh, int64_t lddh, const void* x, int64_t ldx,
@@ -200,8 +202,10 @@ int artlite_gated_ffn_backward(int dtype, int activation, const void* dh, int64_
   a.F = n_ffn;
   AL_TRY(dense_status(dev, &a.status));
   if (!dx && !dw_gate) return ARTLITE_OK;
-  AL_TRY(dtype == ARTLITE_BF16 ? launch_gate_grad<__nv_bfloat16>(a, st) : launch_gate_grad<__half>(a, st));
-  return launch_ffn_backward_gemm(a, st);
+  int rc = dtype == ARTLITE_BF16 ? launch_gate_grad<__nv_bfloat16>(a, st) : launch_gate_grad<__half>(a, st);
+  if (rc == ARTLITE_OK) rc = launch_ffn_backward_gemm(a, st);
+  if (rc == ARTLITE_ECUDA) cudaGetLastError();
+  return rc;
 }
 
 #pragma GCC visibility pop

@@ -57,12 +57,8 @@ struct Smem {
 };
 
 // shared memory: sa stages of A, b_stages of B (width / 2 rows), raw_chunks of packed tiles; as many stages of A as fit
-#ifndef R256
-#define R256 3
-#define RN 6
-#endif
 constexpr int b_stages(int width) { return width == 256 ? 2 : SB_MAX; }  // (a multiple of the sets)
-constexpr int raw_chunks(int width) { return width == 256 ? R256 : RN; }
+constexpr int raw_chunks(int width) { return width == 256 ? 3 : R_MAX; }
 template <int QT>
 constexpr int fixed_bytes(int width) {
   return 1024 + b_stages(width) * (width / 2) * KS * 2 + raw_chunks(width) * (width / 32) * tile_bytes(QT) + (int)sizeof(Smem) +
@@ -445,9 +441,10 @@ int make_tile_map(CUtensorMap* m, const void* base, bool f32, int64_t cols, int6
 
 // The width of a tile: rounds of tiles over the card's pairs times a stage's cycles. Few tokens give few tiles, and narrow
 // ones then keep more of the SMs at work; wide ones read a token row less often and decode for more MMAs. Cycles a stage
-// from measured launches (64: A's copies, 128: the MMAs and copies, 256: the MMAs and the decoding).
+// from measured launches (us at 64 x 4096 x 4096 Q4_0 with 256, 128, 64 columns: 29.1, 19.6, 16.7; at 512 x 4096 x 4096
+// 30.5, 21.3, 27.9; at 1024 x 4096 x 4096 35.1, 37.8, 51.7).
 int width_for(int64_t tm, int64_t N, int per, int pairs) {
-  constexpr int kWidth[] = {256, 128, 64}, kCycles[] = {1250, 750, 600};
+  constexpr int kWidth[] = {256, 128, 64}, kCycles[] = {1250, 730, 570};
   int best = 256;
   int64_t best_cost = -1;
   for (int i = 0; i < 3; i++) {

@@ -11,6 +11,7 @@ from ._lib import QTYPES, Error, LinearDesc, check, lib
 from .moe.block import _ptr
 
 ACTIVATIONS = {"silu": 0, "gelu": 1}
+_BLOCKS = {"Q4_0": (32, 18), "Q4_1": (32, 20), "Q4_K": (256, 144), "IQ4_NL": (32, 18)}  # values, bytes a block
 ACT_DTYPES = {"f32": "F32", "f16": "F16", "bf16": "BF16"}
 
 
@@ -28,6 +29,11 @@ class QuantLinear:
         self._h = None
         self.n_in, self.n_out, self.act = n_in, n_out, act_dtype
         keep = [np.ascontiguousarray(a) if isinstance(a, np.ndarray) else a for a in (w, up)]
+        if qtype in _BLOCKS and n_in > 0 and n_out > 0 and n_in % _BLOCKS[qtype][0] == 0:
+            need = n_in // _BLOCKS[qtype][0] * _BLOCKS[qtype][1] * n_out
+            for a in keep:
+                if getattr(a, "nbytes", need) != need:
+                    raise Error(f"linear: {a.nbytes} bytes of weights, {n_out} {qtype} rows of {n_in} values are {need}")
         d = LinearDesc(n_in=n_in, n_out=n_out, qtype=QTYPES[qtype], act_dtype=QTYPES[ACT_DTYPES[act_dtype]],
                        activation=ACTIVATIONS[activation], device=device)
         h = ctypes.c_void_p()
@@ -52,7 +58,8 @@ class QuantLinear:
     def forward_ptr(self, x, y, T: int, *, ldx: int | None = None, ldy: int | None = None, stream: int = 0) -> None:
         """The product on device buffers (addresses, or objects with ``data_ptr()``): T rows of x ``ldx`` values apart
         (default n_in) and of y ``ldy`` apart (default n_out); enqueued on ``stream`` (0: the device's default)."""
-        rc = self._forward(self._h, _ptr(x), ldx or self.n_in, _ptr(y), ldy or self.n_out, T, stream or None)
+        rc = self._forward(self._h, _ptr(x), self.n_in if ldx is None else ldx, _ptr(y),
+                           self.n_out if ldy is None else ldy, T, stream or None)
         if rc:
             check(rc)
 

@@ -6,7 +6,7 @@ import pytest
 from artlite_b200 import Error, ffn
 from artlite_b200.linear import QuantLinear
 
-W = np.zeros((16, 144), np.uint8)
+W = np.zeros((16, 144), np.uint8)  # (16 Q4_K rows of 256 values)
 
 
 def test_linear_refuses_types_it_does_not_read():
@@ -77,3 +77,11 @@ def test_ffn_work_bytes():
     assert ffn.gated_ffn_work_bytes(5, 64) == 2 * 5 * 64 * 2
     assert ffn.gated_ffn_work_bytes(0, 64) == 0
     assert ffn.gated_ffn_work_bytes(1 << 20, 1 << 14) == 4 << 34  # (past 32 bits)
+
+
+def test_linear_refuses_weights_of_another_size():
+    for w in (W[:15], np.zeros((16, 143), np.uint8), np.zeros((17, 144), np.uint8)):
+        with pytest.raises(Error, match="bytes of weights"):
+            QuantLinear(w, n_in=256, n_out=16, qtype="Q4_K")
+        with pytest.raises(Error, match="bytes of weights"):
+            QuantLinear(W, up=w, n_in=256, n_out=16, qtype="Q4_K")
