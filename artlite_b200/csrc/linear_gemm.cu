@@ -83,6 +83,12 @@ __device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t b
 __device__ __forceinline__ __half2 h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
 __device__ __forceinline__ uint32_t u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 
+// Whether a weight is computed in fp32 and rounded once: Q4_K's scale and minimum (fp16 times six bits) do not fit fp16.
+// For bf16 results they are rounded to it (2^-12 of each; measured 0.0019 of a gated result's norm against 0.0017), for
+// fp16 ones that would cost several times the result's own rounding (0.0010 against 0.0002; in fp32 0.0004).
+template <int QT, class T>
+constexpr bool exact_scales() { return QT == ARTLITE_Q4_K && __is_same(T, __half); }
+
 // A chunk's scales of rows g and g + 8, kept in registers for its four units; of(u, j, ...): unit u's scale (and minimum)
 // of group j, both rows in a pair
 template <int QT>
@@ -104,8 +110,7 @@ struct Scales {
   __half2 dd, dm;
   __device__ __forceinline__ void of(int u, int j, __half2& d, __half2& m) const {
     if constexpr (QT == ARTLITE_Q4_K) {
-      // the file's fp16 and 6-bit scales multiplied in fp16, one rounding: 2^-12 of a weight, against the output's 2^-9 in
-      // bf16. 1024 + s by one logic operation each, both rows at a time
+      // the file's fp16 and 6-bit scales multiplied in fp16; 1024 + s by one logic operation each, both rows at a time
       const uint4 v = make_uint4(j ? w[4] : w[0], j ? w[5] : w[1], j ? w[6] : w[2], 0);
       const uint32_t k = k_fields(v, u);
       const uint32_t s = (k & 0x3Fu) | ((k << 4) & 0x003F0000u) | 0x64006400u;
@@ -120,6 +125,16 @@ struct Scales {
     }
   }
 };
+
+// the same in fp32 (Q4_K): scale and minimum of group j, row g (.x) and g + 8 (.y)
+template <int QT>
+__device__ __forceinline__ void scales32(const Scales<QT>& sc, int u, int j, float2& d, float2& m) {
+  const uint4 v = make_uint4(j ? sc.w[4] : sc.w[0], j ? sc.w[5] : sc.w[1], j ? sc.w[6] : sc.w[2], 0);
+  const uint32_t k = k_fields(v, u);
+  const float2 dd = __half22float2(sc.dd), dm = __half22float2(sc.dm);
+  d.x = fmaf(k_field(k, 0), dd.x, -8388608.0f * dd.x), d.y = fmaf(k_field(k, 12), dd.y, -8388608.0f * dd.y);
+  m.x = fmaf(k_field(k, 6), dm.x, -8388608.0f * dm.x), m.y = fmaf(k_field(k, 18), dm.y, -8388608.0f * dm.y);
+}
 
 // a word's eight values times their group's scale: one rounding to fp16 from the exact codes. A nibble in a half's bits
 // 0 - 3 under 0x6400 is 1024 + q, in bits 4 - 7 it is 1024 + 16 q; the offset is taken away exactly, and for the latter
@@ -144,6 +159,20 @@ __device__ __forceinline__ uint4 decode8(uint32_t w, __half2 d, __half2 m, const
     }
     return make_uint4(o[0], o[1], o[2], o[3]);
   }
+}
+
+// the same with an fp32 scale and minimum, one rounding
+__device__ __forceinline__ uint4 decode8_32(uint32_t w, float d, float m) {
+  uint32_t o[4];
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const uint32_t v = h ? w >> 8 : w;
+    const float2 a = __half22float2(__hsub2(h2((v & 0x000F000Fu) | 0x64006400u), h2(0x64006400u)));
+    const float2 b = __half22float2(__hfma2(h2((v & 0x00F000F0u) | 0x64006400u), h2(0x2C002C00u), h2(0xD400D400u)));
+    o[2 * h] = u32(__floats2half2_rn(fmaf(a.x, d, m), fmaf(a.y, d, m)));
+    o[2 * h + 1] = u32(__floats2half2_rn(fmaf(b.x, d, m), fmaf(b.y, d, m)));
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 template <int QT, class T, bool GATED>
@@ -300,10 +329,17 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
             const uint32_t w[2][2] = {{odd ? w4.z : w4.x, odd ? w4.x : w4.z}, {odd ? w4.w : w4.y, odd ? w4.y : w4.w}};
 #pragma unroll
             for (int jj = 0; jj < 2; jj++) {
-              __half2 d, m;
-              sc.of(2 * h + v, jj ^ odd, d, m);
-              c[v][0][jj] = decode8<QT>(w[0][jj], __low2half2(d), __low2half2(m), table);
-              c[v][1][jj] = decode8<QT>(w[1][jj], __high2half2(d), __high2half2(m), table);
+              if constexpr (exact_scales<QT, T>()) {
+                float2 d, m;
+                scales32(sc, 2 * h + v, jj ^ odd, d, m);
+                c[v][0][jj] = decode8_32(w[0][jj], d.x, m.x);
+                c[v][1][jj] = decode8_32(w[1][jj], d.y, m.y);
+              } else {
+                __half2 d, m;
+                sc.of(2 * h + v, jj ^ odd, d, m);
+                c[v][0][jj] = decode8<QT>(w[0][jj], __low2half2(d), __low2half2(m), table);
+                c[v][1][jj] = decode8<QT>(w[1][jj], __high2half2(d), __high2half2(m), table);
+              }
             }
           }
           if (!tc::wait(&sm->abort, &sm->empty_b[s], ph ^ 1, p.status, 46)) goto out;

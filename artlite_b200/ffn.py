@@ -2,19 +2,20 @@
 ``artlite_gated_ffn_backward``, include/artlite_moe.h), on the caller's device buffers: addresses, or objects with
 ``data_ptr()``. For 4-bit GGUF matrices: ``artlite_b200.linear.QuantLinear`` with ``up``."""
 
-import ctypes
-
 from ._lib import QTYPES, Error, check, lib
-from .linear import ACTIVATIONS
-from .moe.block import _ptr
+from .linear import ACTIVATIONS, _ptr
 
 DTYPES = {"f16": "F16", "bf16": "BF16"}
 
 
+_CODES = {(d, a): (QTYPES[t], n) for d, t in DTYPES.items() for a, n in ACTIVATIONS.items()}
+
+
 def _codes(dtype: str, activation: str) -> tuple[int, int]:
-    if dtype not in DTYPES or activation not in ACTIVATIONS:
+    codes = _CODES.get((dtype, activation))
+    if codes is None:
         raise Error(f"gated_ffn: type {dtype}, activation {activation}")
-    return QTYPES[DTYPES[dtype]], ACTIVATIONS[activation]
+    return codes
 
 
 def gated_ffn(x, w_gate, w_up, h, *, T: int, n_in: int, n_ffn: int, dtype: str = "bf16", activation: str = "silu",
@@ -22,9 +23,11 @@ def gated_ffn(x, w_gate, w_up, h, *, T: int, n_in: int, n_ffn: int, dtype: str =
     """h (T, n_ffn) = act(x w_gate^T) * (x w_up^T) of x (T, n_in) and w_gate, w_up (n_ffn, n_in); ``gate``, ``up`` (T,
     n_ffn) fp32: the two products, kept for ``gated_ffn_backward``. ``ldx``, ``ldh``: values between rows."""
     dt, act = _codes(dtype, activation)
-    check(lib().artlite_gated_ffn(dt, act, _ptr(x), n_in if ldx is None else ldx, _ptr(w_gate), _ptr(w_up), _ptr(h),
-                                  n_ffn if ldh is None else ldh, _ptr(gate), _ptr(up), T, n_in, n_ffn,
-                                  ctypes.c_void_p(stream or None)))
+    rc = lib().artlite_gated_ffn(dt, act, _ptr(x), n_in if ldx is None else ldx, _ptr(w_gate), _ptr(w_up), _ptr(h),
+                                 n_ffn if ldh is None else ldh, None if gate is None else _ptr(gate),
+                                 None if up is None else _ptr(up), T, n_in, n_ffn, stream or None)
+    if rc:
+        check(rc)
 
 
 def gated_ffn_work_bytes(T: int, n_ffn: int) -> int:
@@ -41,4 +44,4 @@ def gated_ffn_backward(dh, x, w_gate, w_up, gate, up, work, *, T: int, n_in: int
     check(lib().artlite_gated_ffn_backward(dt, act, _ptr(dh), n_ffn if lddh is None else lddh, _ptr(x),
                                            n_in if ldx is None else ldx, _ptr(w_gate), _ptr(w_up), _ptr(gate), _ptr(up),
                                            _ptr(work), _ptr(dx), n_in if lddx is None else lddx, _ptr(dw_gate),
-                                           _ptr(dw_up), T, n_in, n_ffn, ctypes.c_void_p(stream or None)))
+                                           _ptr(dw_up), T, n_in, n_ffn, stream or None))

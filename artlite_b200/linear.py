@@ -8,11 +8,19 @@ import ctypes
 import numpy as np
 
 from ._lib import QTYPES, Error, LinearDesc, check, lib
-from .moe.block import _ptr
+from .moe.block import _ptr as _any_ptr
 
 ACTIVATIONS = {"silu": 0, "gelu": 1}
 _BLOCKS = {"Q4_0": (32, 18), "Q4_1": (32, 20), "Q4_K": (256, 144), "IQ4_NL": (32, 18)}  # values, bytes a block
 ACT_DTYPES = {"f32": "F32", "f16": "F16", "bf16": "BF16"}
+
+
+def _ptr(a) -> int | None:
+    """``moe.block._ptr``, device tensors first: the calls here take a few microseconds and so would its checks."""
+    try:
+        return a.data_ptr()
+    except AttributeError:
+        return _any_ptr(a)
 
 
 class QuantLinear:
