@@ -295,19 +295,22 @@ int pack(artlite_linear* h, int which, const void* raw) {
   const int qt = h->d.qtype, K = h->d.n_in;
   const int64_t N = h->d.n_out;
   const int64_t rb = (int64_t)K / q_per(qt) * q_bytes(qt);
-  DevBuf stage, bound;
+  DevBuf stage;
   const uint8_t* src = static_cast<const uint8_t*>(raw);
   if (device_of(raw) != h->dev) {
     AL_TRY(stage.reserve((size_t)(N * rb)));
     AL_CUDA(cudaMemcpy(stage.ptr, raw, (size_t)(N * rb), cudaMemcpyDefault));
     src = stage.as<uint8_t>();
   }
-  AL_TRY(bound.reserve(4));
-  AL_CUDA(cudaMemset(bound.ptr, 0, 4));
-  weight_bound_kernel<<<1024, 256>>>(qt, src, rb, N, K, bound.as<uint32_t>());
+  AL_CUDA(cudaDeviceSynchronize());  // (device rows may still be written on a stream of the caller's)
+  void* bound;
+  AL_TRY(stream_alloc(h->dev, sizeof(float), nullptr, &bound));
+  AL_CUDA(cudaMemsetAsync(bound, 0, sizeof(float), nullptr));
+  weight_bound_kernel<<<1024, 256>>>(qt, src, rb, N, K, static_cast<uint32_t*>(bound));
   AL_LAUNCHED();
   float m;
-  AL_CUDA(cudaMemcpy(&m, bound.ptr, 4, cudaMemcpyDeviceToHost));
+  AL_CUDA(cudaMemcpy(&m, bound, sizeof(float), cudaMemcpyDeviceToHost));
+  AL_TRY(stream_free(bound, nullptr));
   // the prompt kernel multiplies the scales by 2^w_exp: the largest weight then lies below 2^15 in fp16, and only those
   // 2^-29 below it lose bits (a matrix whose largest is under 2^-14 stays smaller than that)
   if (m > 0.0f && isfinite(m)) h->w_exp[which] = std::min(std::max(14 - ilogbf(m), -14), 28);
