@@ -100,7 +100,7 @@ inline int make_operand_map(CUtensorMap* m, const void* base, int64_t cols, int6
   return make_tile_map(m, base, false, cols, rows, ld, box_x, box_y);
 }
 
-// a programmatic launch of `pairs` CTA pairs (the kernel calls griddep_wait before it touches memory)
+// a launch of `pairs` CTA pairs; an ordinary one (small_batch.cuh says why not a programmatic one)
 template <class K, class P>
 int launch_pairs(K kern, const P& p, int pairs, int threads, size_t smem, cudaStream_t st) {
   AL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
@@ -109,15 +109,13 @@ int launch_pairs(K kern, const P& p, int pairs, int threads, size_t smem, cudaSt
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[2];
+  cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  cfg.numAttrs = 1;
   AL_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
   count_launch();
   return ARTLITE_OK;

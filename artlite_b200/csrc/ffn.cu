@@ -16,8 +16,6 @@ namespace {
 template <class T>
 __global__ void gate_grad_kernel(const T* dh, int64_t lddh, const float* g, const float* u, int act, int64_t T_, int F,
                                  T* dg, T* du) {
-  griddep_launch();
-  griddep_wait();
   const int per = F / 8;
   const int64_t n = T_ * per;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
@@ -49,8 +47,10 @@ template <class T>
 int launch_gate_grad(const FfnArgs& a, cudaStream_t st) {
   const int64_t n = a.T * (a.F / 8);
   const unsigned grid = (unsigned)min64(cdiv(n, 256), 1 << 20);
-  return launch_pdl(gate_grad_kernel<T>, dim3(grid), dim3(256), 0, st, static_cast<const T*>(a.dh), a.lddh, a.g, a.u, a.act,
-                    a.T, a.F, static_cast<T*>(a.dg), static_cast<T*>(a.du));
+  gate_grad_kernel<T><<<grid, 256, 0, st>>>(static_cast<const T*>(a.dh), a.lddh, a.g, a.u, a.act, a.T, a.F,
+                                            static_cast<T*>(a.dg), static_cast<T*>(a.du));
+  AL_LAUNCHED();
+  return ARTLITE_OK;
 }
 
 // tokens up to which the small-batch kernel runs. Measured at 2048 x 6144 bf16 (us), small batch and tensor-core tiles:

@@ -92,7 +92,6 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
   const int total = p.job[0].tiles + (MODE == kBackward ? p.job[1].tiles : 0);
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
-  griddep_launch();
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; i++) {
       tc::mbar_init(&sm->full[i], 1);
@@ -110,7 +109,6 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm(const __grid_constant__ 
   tc::cluster_sync();
   tc::fence_after();
   const uint32_t tmem = sm->tmem_base;
-  griddep_wait();
 
   if (warp == 0 && lane == 0) {
     // ---------------- TMA: this CTA's halves of A and B

@@ -213,8 +213,6 @@ __global__ void pack_kernel(int qt, const uint8_t* raw, int64_t rb, int64_t N, i
 // x's rows as scaled fp16 (linear.cuh): a CTA a row, whose first 8192 values stay in registers between the search for the
 // largest and the scaling
 __global__ void __launch_bounds__(256) half_rows_kernel(const uint16_t* x, int64_t ldx, int K, uint16_t* out, int32_t* row_exp) {
-  griddep_launch();
-  griddep_wait();
   const uint16_t* row = x + (int64_t)blockIdx.x * ldx;
   __shared__ float part[8];
   constexpr int kHeld = 4, kStep = 8 * 256;
@@ -270,7 +268,9 @@ bool linear_type(int qt) {
 }  // namespace
 
 int launch_half_rows(const uint16_t* x, int64_t ldx, int64_t T, int K, uint16_t* out, int32_t* row_exp, cudaStream_t st) {
-  return launch_pdl(half_rows_kernel, dim3((unsigned)T), dim3(256), 0, st, x, ldx, K, out, row_exp);
+  half_rows_kernel<<<(unsigned)T, 256, 0, st>>>(x, ldx, K, out, row_exp);
+  AL_LAUNCHED();
+  return ARTLITE_OK;
 }
 
 }  // namespace artlite

@@ -193,7 +193,6 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
   const int total = p.order.tm * p.order.tn, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int ksteps = (p.K + KS - 1) / KS, chunks = (p.K + kTileK - 1) / kTileK;
 
-  griddep_launch();
   if (threadIdx.x == 0) {
     for (int i = 0; i < SA; i++) {
       tc::mbar_init(&sm->full_a[i], 1);
@@ -224,7 +223,6 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
   tc::cluster_sync();
   tc::fence_after();
   const uint32_t tmem = sm->tmem_base;
-  griddep_wait();
 
   if (warp == 0 && lane == 0) {
     // ---------------- the token rows (each CTA its 128)

@@ -28,9 +28,10 @@ namespace sb {
 
 constexpr int kWarps = 16, kThreads = 32 * kWarps;
 constexpr int kMaxCluster = 8;
-// One CTA an SM: with two, a launch that starts while the one before it ends finds some SMs half free and others not, and
-// puts two of its CTAs on the former (measured: 11 us become 25). So a CTA always takes more than half of an SM's memory.
-constexpr int kSmemMax = 227 * 1024, kSmemMin = 120 * 1024;
+// One CTA an SM. The launches are ordinary ones: as programmatic dependent launches (which measured 1 us less a call back
+// to back) a chain of this library's cluster kernels stopped for good on the device (a training step's three kernels,
+// queued a thousand deep), and the reason was not found.
+constexpr int kSmemMax = 227 * 1024;
 // Bytes a CTA keeps in flight: more of them only queue. Measured with 16-bit weights of 50 MB, T = 1: 64 KB 11.1 us, 72 KB
 // 10.9, 128 KB 12.9 - 16, 196 KB 17.0
 constexpr int kInFlight = 74 * 1024;
@@ -624,7 +625,6 @@ __global__ void __launch_bounds__(kThreads, 1) small_batch(const __grid_constant
   float* red = reinterpret_cast<float*>(sm + a.plan.red_off);
   const bool works = tl < tp && it0 + kl < it1;
 
-  griddep_launch();
   float* scale = reinterpret_cast<float*>(abort + 2);
   uint32_t* top = reinterpret_cast<uint32_t*>(scale + 8);
   if (threadIdx.x == 0) *abort = 0;
@@ -643,13 +643,10 @@ __global__ void __launch_bounds__(kThreads, 1) small_batch(const __grid_constant
       if (ri >= it1) ri = it0 + kl, rt += tp;
     }
   };
-  // (a 4-bit matrix is never written after its handle was made: its first items may come before the kernels ahead of
-  // this one have ended)
-  if constexpr (S::kPlain) griddep_wait();
+  // (the first items are on their way while x is laid out)
   if (works && lane == 0)
     for (int i = 0; i < a.plan.depth; i++) request(i);
   if constexpr (S::kInt) __syncthreads();
-  if constexpr (!S::kPlain) griddep_wait();
 
   const uint32_t* table = nullptr;
   if constexpr (S::kTable) {  // a copy of the table for every lane: reads without bank conflicts
@@ -851,7 +848,7 @@ bool plan_for(const Args& a, int per, int cols, const int* max_clusters, Plan* b
       off += (int)red;
       best->bar_off = off;
       off += kWarps * depth * 8 + 128;  // (the barriers; the abort word; QuantInt's scales and largest values)
-      best->smem = off + 1024 > kSmemMin ? off + 1024 : kSmemMin;
+      best->smem = off + 1024;
     }
   }
   return best_cost >= 0;
@@ -934,15 +931,13 @@ int launch_one(const Args& args, int dev, cudaStream_t st, bool* planned) {
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = (size_t)p.smem;
     cfg.stream = st;
-    cudaLaunchAttribute at[2];
+    cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned)p.c;
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    cfg.numAttrs = 1;
     AL_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
     count_launch();
   }
