@@ -28,21 +28,21 @@ __device__ __forceinline__ void tile_at(const TileOrder& o, int id, int* m, int*
   *m = grp * G + (rem - *n * gm);
 }
 
-// 16 consecutive values of an output row: 16-byte stores where the row allows them (vec) and all are inside
+// 16 consecutive values of an output row that takes 16-byte stores, those below `valid`
 template <class T>
-__device__ __forceinline__ void store16(T* dst, const float (&v)[16], int valid, bool vec) {
-  if (valid <= 0) return;
-  if (vec && valid >= 16) {
+__device__ __forceinline__ void store16(T* dst, const float (&v)[16], int valid) {
 #pragma unroll
-    for (int c = 0; c < 2; c++)
+  for (int c = 0; c < 2; c++) {
+    if (valid >= 8 * c + 8) {
       reinterpret_cast<uint4*>(dst)[c] =
           make_uint4(Num<T>::pack(v[8 * c], v[8 * c + 1]), Num<T>::pack(v[8 * c + 2], v[8 * c + 3]),
                      Num<T>::pack(v[8 * c + 4], v[8 * c + 5]), Num<T>::pack(v[8 * c + 6], v[8 * c + 7]));
-    return;
-  }
+    } else {
 #pragma unroll
-  for (int j = 0; j < 16; j++)
-    if (j < valid) dst[j] = Num<T>::down(v[j]);
+      for (int j = 8 * c; j < 8 * c + 8; j++)
+        if (j < valid) dst[j] = Num<T>::down(v[j]);
+    }
+  }
 }
 
 // A warp's 32 x 32 output chunk by TMA: lane l's row l into a 4 KB shared-memory slot in the map's swizzle, then one

@@ -341,7 +341,7 @@ int small_of(int qt, const sb::Args& a, bool gated, int dev, cudaStream_t st) {
 }
 
 // tokens up to which the small-batch kernel runs. Measured (us) against tensor-core tiles: 4096 x 4096 Q4_0 T = 16
-// 10.9 / 17, 32 14.3 / 17, 48 26 / 17; 2048 x 8192 Q4_K T = 32 17.9 / 14, 24 16.6 / 14, 16 11.4 / 14
+// 11.9 / 17.8, 32 15.0 / 17.7, 48 26.8 / 17.8; 2048 x 8192 Q4_K T = 16 12.6 / 19.0, 32 18.7 / 15.3, 48 33.1 / 15.4
 constexpr int64_t kSmallTokens = 32;
 
 int run(const artlite_linear* h, const void* x, int64_t ldx, void* y, int64_t ldy, int64_t T, cudaStream_t st) {

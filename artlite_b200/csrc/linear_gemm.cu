@@ -15,6 +15,11 @@
 //
 // Warps: 0 the token rows' TMA, 1 the MMAs (the leader CTA's), 2 the packed tiles' copies, 3 idle, 4 - 7 the epilogue,
 // 8 - 15 the decoding.
+//
+// What bounds it: the decoding. A stage of 128 values takes 1024 cycles of MMAs, and a decoding warp about 1260 from one
+// stage to the next (470 of arithmetic; Q4_K 680, the rest waits, stores, the proxy fence and the arrival, in turn). 4000 x
+// 4096 x 4096 Q4_0 119 us (1.13 PFLOP/s, the tensor pipe 74% active; 256 tiles on 74 pairs leave 14% of it idle), 2048 x
+// 2048 x 6144 gated Q4_K 98 us (67%). A second set of decoding warps, deeper rings and wider copies changed nothing.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -54,6 +59,7 @@ struct Smem {
   uint64_t full_a[SA_MAX], empty_a[SA_MAX], full_b[SB_MAX], empty_b[SB_MAX], raw_full[R_MAX], raw_empty[R_MAX], tfull[2], tempty[2];
   uint32_t tmem_base;
   int abort;
+  uint16_t out[4][32][18];  // an epilogue warp's 32 x 16 results, for rows that no 16-byte store takes
 };
 
 // shared memory: sa stages of A, b_stages of B (width / 2 rows), raw_chunks of packed tiles; as many stages of A as fit
@@ -397,7 +403,24 @@ __global__ void __launch_bounds__(kThreads, 1) linear_gemm(const __grid_constant
 #pragma unroll
           for (int j = 0; j < 16; j++) o[j] = __uint_as_float(v[j]) * a0 * a1;
         }
-        if (live) store16<T>(row + f, o, p.N - f, p.vec_y);
+        if (p.vec_y) {
+          if (live) store16<T>(row + f, o, p.N - f);
+        } else {
+          // (by way of shared memory: 16 lanes store 32 consecutive bytes of a row, where a lane a row would touch 32 lines
+          // with every two bytes)
+#pragma unroll
+          for (int j = 0; j < 16; j += 2)
+            *reinterpret_cast<uint32_t*>(&sm->out[q][lane][j]) = Num<T>::pack(o[j], o[j + 1]);
+          __syncwarp();
+          const int first = tok - lane;
+#pragma unroll
+          for (int j = 0; j < 16; j++) {
+            const int r = 2 * j + (lane >> 4), col = f + (lane & 15);
+            if (first + r < p.T && col < p.N)
+              reinterpret_cast<uint16_t*>(p.y)[(int64_t)(first + r) * p.ldy + col] = sm->out[q][r][lane & 15];
+          }
+          __syncwarp();
+        }
       }
       tc::fence_before();
       __syncwarp();

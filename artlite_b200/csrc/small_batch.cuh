@@ -289,7 +289,9 @@ struct Quant {
   }
 };
 
-// The same tiles for one to four tokens (NT of them), on the integer MMA: a token takes all eight columns.
+// The same tiles for one, two or four tokens (NT of them), on the integer MMA: a token takes all eight columns. What bounds
+// one token: 2048 x 8192 gated Q4_K reads 18.9 MB in 8.6 us (2.2 TB/s; its copies alone take 5 us, the decoding and the two
+// MMAs a unit the rest), where multiplying every group in fp16 fragments took 11.
 //
 // x becomes 32-bit fixed point over the CTA's values (2^k x, the largest in [2^29, 2^30): what is 2^-30 of a row's largest
 // and less is lost, under fp32's own rounding of such a sum) and its four signed 8-bit digits four columns; the unit's two
@@ -950,13 +952,14 @@ template <class S, class XT, bool GATED>
 int launch(const Args& args, int dev, cudaStream_t st) {
   Args a = args;
   if constexpr (!S::kPlain && !S::kTable) {
-    // one to four tokens: the integer MMA. Measured at T = 1, 2, 4, 8 (us): see linear.cu
-    if (a.T <= 4) {
-      bool planned;
+    // One or two tokens (fp32: four, whose other way takes three MMAs a step): the integer MMA. Measured (us) at 4096 x 4096
+    // Q4_0 and 2048 x 8192 Q4_K: T = 1 6.3 and 6.5, 2 8.4 and 7.7, 4 11.7 and 10.0; the other way at T = 8 9.1 and 9.5
+    if (a.T <= (sizeof(XT) == 4 ? 4 : 2)) {
+      bool planned = false;
       a.group = a.T <= 2 ? (int)a.T : 4;
-      AL_TRY((a.group == 1   ? launch_one<typename S::Int, XT, 1, GATED>(a, dev, st, &planned)
-              : a.group == 2 ? launch_one<typename S::Int, XT, 2, GATED>(a, dev, st, &planned)
-                             : launch_one<typename S::Int, XT, 4, GATED>(a, dev, st, &planned)));
+      if (a.group == 1) AL_TRY((launch_one<typename S::Int, XT, 1, GATED>(a, dev, st, &planned)));
+      else if (a.group == 2) AL_TRY((launch_one<typename S::Int, XT, 2, GATED>(a, dev, st, &planned)));
+      else if constexpr (sizeof(XT) == 4) AL_TRY((launch_one<typename S::Int, XT, 4, GATED>(a, dev, st, &planned)));
       if (planned) return ARTLITE_OK;
     }
   }
