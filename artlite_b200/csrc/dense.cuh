@@ -11,7 +11,7 @@
 
 namespace artlite {
 
-enum { kActNone = -1, kActSilu = 0, kActGelu = 1 };
+enum { kActSilu = ARTLITE_ACT_SILU, kActGelu = ARTLITE_ACT_GELU };
 
 // ---------------------------------------------------------------- activations
 //
@@ -56,7 +56,6 @@ template <class T>
 struct Num;
 template <>
 struct Num<__nv_bfloat16> {
-  static __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -68,7 +67,6 @@ struct Num<__nv_bfloat16> {
 };
 template <>
 struct Num<__half> {
-  static __device__ __forceinline__ float up(__half v) { return __half2float(v); }
   static __device__ __forceinline__ __half down(float v) { return __float2half_rn(v); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
@@ -80,7 +78,6 @@ struct Num<__half> {
 };
 template <>
 struct Num<float> {
-  static __device__ __forceinline__ float up(float v) { return v; }
   static __device__ __forceinline__ float down(float v) { return v; }
 };
 

@@ -253,11 +253,13 @@ int artlite_linear_create(const artlite_linear_desc* desc, const void* w, const 
 
 /*
  * y (T rows, ldy values apart) = x (T rows, ldx values apart) . w^T, or with w_up act(x . w^T) * (x . w_up^T). Sums in
- * fp32. Up to 32 tokens, and any number of fp32 or unaligned ones: the products are exact and only the sums and the
- * result round. Above (16-bit x with 16-byte aligned rows): each weight, and a bf16 x after scaling its row by a power of
- * two, enters the tensor cores as fp16. An infinity or NaN in x makes that token's row of y NaN or infinite. x and y are
- * both device memory of the handle's device, or both host memory (staged; the call returns when y is back). The handle
- * keeps no state between calls: calls may overlap on any streams and in any captured graphs.
+ * fp32. Up to 32 tokens, and any number of fp32 or unaligned ones: the weights are exact and only the sums and the result
+ * round; for one or two tokens (fp32: four) x is held as 32-bit fixed point, which loses what is 2^-30 of a row's largest
+ * value and less. Above 32 tokens (16-bit x with 16-byte aligned rows): each weight, and a bf16 x after scaling its row by
+ * a power of two, enters the tensor cores as fp16; a bf16 x then takes 2 T n_in bytes of scratch from a pool of this
+ * library's (inside a capture: the graph's own memory). An infinity or NaN in x makes that token's row of y NaN or
+ * infinite. x and y are both device memory of the handle's device, or both host memory (staged; the call returns when y is
+ * back). The handle keeps no state between calls: calls may overlap on any streams and in any captured graphs.
  */
 int artlite_linear_forward(const artlite_linear* h, const void* x, int64_t ldx, void* y, int64_t ldy, int64_t T,
                            void* stream);
