@@ -728,18 +728,19 @@ __global__ void __launch_bounds__(kThreads, 1) small_batch(const __grid_constant
       }
     }
     __syncthreads();
-    // the batch's sums: this CTA's warps' in order (into the first's place), then the cluster's CTAs' in order
+    // the batch's sums: this CTA's warps' in order (in a cluster into the first's place), then the cluster's CTAs' in order
     const int n_it = it1 - it0, nk = min(a.plan.wk, n_it);
-    for (int o = threadIdx.x; o < (b1 - b0) * cols * 16; o += kThreads) {
-      const int r = o & 15, tc_ = o >> 4, col = tc_ % cols, lt = tc_ / cols;
-      float* p = red + lt * a.plan.wk * partial + col * kCol + r;
-      float v = p[0];
+    if (c > 1) {
+      for (int o = threadIdx.x; o < (b1 - b0) * cols * 16; o += kThreads) {
+        const int r = o & 15, tc_ = o >> 4, col = tc_ % cols, lt = tc_ / cols;
+        float* p = red + lt * a.plan.wk * partial + col * kCol + r;
+        float v = p[0];
 #pragma unroll 4
-      for (int k = 1; k < nk; k++) v += p[k * partial];
-      p[0] = v;
+        for (int k = 1; k < nk; k++) v += p[k * partial];
+        p[0] = v;
+      }
+      tc::cluster_sync();
     }
-    if (c > 1) tc::cluster_sync();
-    else __syncthreads();
     const int rows = (b1 - b0) / kPer * 16, outs = rows * cols;
     for (int o = threadIdx.x + kThreads * rank; o < outs; o += kThreads * c) {
       const int r = o % rows, col = o / rows, lt = r >> 4;
@@ -749,6 +750,8 @@ __global__ void __launch_bounds__(kThreads, 1) small_batch(const __grid_constant
         const float* p = red + (kPer * lt + m) * a.plan.wk * partial + col * kCol + (r & 15);
         if (c == 1) {
           v[m] = p[0];
+#pragma unroll 4
+          for (int k = 1; k < nk; k++) v[m] += p[k * partial];
         } else {
           float part[kMaxCluster];
 #pragma unroll
@@ -776,7 +779,7 @@ __global__ void __launch_bounds__(kThreads, 1) small_batch(const __grid_constant
       }
     }
     if (c > 1) tc::cluster_sync();  // (the partial sums are free, and no CTA leaves while another reads its)
-    else __syncthreads();
+    else if (b1 < tile1) __syncthreads();
   }
   // (after a wait that ran out: the copies still in flight land before the CTA's memory is given back)
   if (*(volatile int*)abort) {
